@@ -44,9 +44,10 @@ enum {
     TLB_DEV_BAD_BOX = 2u,      /* sample skipped (output zero-filled): box leaves the image */
     TLB_DEV_TOO_WIDE = 4u,     /* sample skipped (output zero-filled): crop exceeds staging */
     TLB_DEV_COPY_TIMEOUT = 8u, /* a bounded wait on an async copy gave up                   */
+    TLB_DEV_BAD_LENGTH = 16u,  /* a sample's length lies outside [0, tokens]: clamped        */
 };
 
-enum { TLB_F32 = 0, TLB_BF16 = 1 };
+enum { TLB_F32 = 0, TLB_BF16 = 1, TLB_F16 = 2 /* microscaled entry points only */ };
 enum { TLB_NCHW = 0, TLB_NHWC = 1 };
 
 /*
@@ -349,6 +350,92 @@ TLB_API tlb_epoch* tlb_epoch_create(const tlb_transform_desc* first, int64_t tot
  * is made to wait for the batch; slots are refilled only behind the work already enqueued on it. */
 TLB_API int tlb_epoch_next(tlb_epoch* e, int64_t* batch, int32_t* n, int32_t* slot, void* consumer_stream);
 TLB_API void tlb_epoch_destroy(tlb_epoch* e);
+
+/* ---- microscaled rows: features, their cache and the products on it ---------------------------
+ * A feature set (the outputs of a frozen image encoder: `tokens` rows of `cols` values a sample) is
+ * held in HBM in 4 or 8 bits a value, written by sample number, served in shuffled order and
+ * multiplied without being widened.  No counterpart in the reference, whose resident loader keeps
+ * uint8 pixels (turboloader/cuda_loader.py:385-535).
+ *
+ * A block of consecutive values of a row shares one 8-bit scale.  With t = fp32(x / tensor scale) and
+ * a = max |t| of the block (roundings to nearest even, saturating):
+ *   TLB_MX_NVFP4  16 values: scale s = e4m3(a / 6),                   codes e2m1(t / s)
+ *   TLB_MX_MXFP4  32 values: scale s = 2^max(floor(log2 a) - 2, -127), codes e2m1(t / s)
+ *   TLB_MX_MXFP8  32 values: scale s = 2^max(floor(log2 a) - 8, -127), codes e4m3(t / s)
+ * An nvfp4 scale that rounds to zero makes its codes zero.  A block that holds an infinity or a NaN
+ * gets a NaN scale and zero codes: all of it reads as NaN.  A code stands for code * s * tensor scale
+ * (code * s is exact in fp32 and in bf16).
+ *
+ * Layout: rows are padded to 128 values; a row of codes takes tlb_mx_code_pitch bytes (4-bit codes: two a
+ * byte, the earlier value in the low half) and a row of scales tlb_mx_scale_pitch bytes, rows packed
+ * without gaps.  Pad codes and pad scale bytes are zero (the calls below write them so, and the products
+ * rely on it). */
+enum { TLB_MX_NVFP4 = 0, TLB_MX_MXFP4 = 1, TLB_MX_MXFP8 = 2 };
+#define TLB_MX_MAX_COLS (1 << 20)
+#define TLB_MX_MAX_ROWS (1ll << 30)
+#define TLB_MX_SCAN_SAMPLES 256
+
+typedef struct tlb_mx_rows {
+    uint8_t* codes;            /* DEVICE, 16-byte aligned                                   */
+    uint8_t* scales;           /* DEVICE, 4-byte aligned                                    */
+    int64_t rows;
+    int32_t cols;              /* values of a row                                           */
+    int32_t format;            /* TLB_MX_*                                                  */
+    float scale;               /* tensor scale = scale * (scale_dev ? *scale_dev : 1);      */
+    const float* scale_dev;    /* scale positive and finite, *scale_dev too (not checked)   */
+} tlb_mx_rows;
+
+TLB_API int64_t tlb_mx_code_pitch(int32_t format, int32_t cols);   /* bytes, or -1 */
+TLB_API int64_t tlb_mx_scale_pitch(int32_t format, int32_t cols);  /* bytes, or -1 */
+
+/* x (rows, cols) of x_dtype, x_pitch elements between rows -> q.  All entry points of this section
+ * enqueue on `stream`, on the current device, allocate nothing, do not synchronise and may be captured
+ * into a CUDA graph. */
+TLB_API int tlb_mx_quantize(const tlb_mx_rows* q, const void* x, int32_t x_dtype, int64_t x_pitch, void* stream);
+
+/* A cache: rows.rows = slots * tokens.  One sample fills one slot. */
+typedef struct tlb_mx_cache {
+    tlb_mx_rows rows;
+    int32_t tokens;            /* rows of a sample                                          */
+    int32_t* lengths;          /* DEVICE [slots] rows in use of every sample, or NULL: all   */
+    int32_t* owner;            /* DEVICE [slots] words, all -1 before the first write (and   */
+                               /*   again after every one); for writes of more than          */
+                               /*   TLB_MX_SCAN_SAMPLES samples, else NULL will do           */
+    uint32_t* status;          /* DEVICE word OR-ed with TLB_DEV_* bits, or NULL             */
+} tlb_mx_cache;
+
+/* Sample i of x (n samples of `tokens` rows; pitches in elements) is quantised into slot index[i]
+ * (DEVICE).  With lengths (DEVICE [n]; the cache then has lengths) only the first lengths[i] rows are
+ * read and written, the slot's other rows stay as they were, and the cache takes the length; without,
+ * the length becomes `tokens`.  A slot named twice takes the last of its samples; an index outside the
+ * cache is skipped and reported (TLB_DEV_BAD_INDEX).  Two writes of one cache that overlap in time
+ * (other streams) may not name the same slot. */
+TLB_API int tlb_mx_write(const tlb_mx_cache* cache, const int64_t* index, int64_t n, const void* x, int32_t x_dtype,
+                         int64_t row_pitch, int64_t sample_pitch, const int32_t* lengths, void* stream);
+/* Samples index[i] (NULL: 0..n-1) as values, (n, tokens, cols) packed: zeros behind a sample's length
+ * and for an index outside the cache (TLB_DEV_BAD_INDEX).  lengths_out (may be NULL): their lengths. */
+TLB_API int tlb_mx_read(const tlb_mx_cache* cache, const int64_t* index, int64_t n, void* out, int32_t out_dtype,
+                        int32_t* lengths_out, void* stream);
+/* The same samples as they are held: codes and scales of n * tokens rows, zero rows where tlb_mx_read
+ * gives zeros. */
+TLB_API int tlb_mx_read_codes(const tlb_mx_cache* cache, const int64_t* index, int64_t n, uint8_t* codes,
+                              uint8_t* scales, int32_t* lengths_out, void* stream);
+
+/* out (a.rows, b.rows) packed = values(a) * values(b)^T, sums in fp32, rounded once.  a and b have the
+ * same format and cols.  workspace: tlb_mx_matmul_workspace bytes (0: NULL will do), 256-byte aligned,
+ * used by this call alone until its work has ended. */
+TLB_API int64_t tlb_mx_matmul_workspace(const tlb_mx_rows* a, const tlb_mx_rows* b, int32_t out_dtype);
+TLB_API int tlb_mx_matmul(const tlb_mx_rows* a, const tlb_mx_rows* b, void* out, int32_t out_dtype, void* workspace,
+                          int64_t workspace_bytes, void* stream);
+
+/* Gradients of that product with respect to the values of an operand, g (m, n) packed:
+ *   transpose = 0: out (m, q.cols) = g * values(q),    q = b (n rows): the gradient of a
+ *   transpose = 1: out (n, q.cols) = g^T * values(q),  q = a (m rows): the gradient of b
+ * Every value of g enters whole (fp32 as the sum of three bf16 terms, fp16 of two); sums in fp32. */
+TLB_API int64_t tlb_mx_grad_workspace(int32_t g_dtype, int64_t m, int32_t n, const tlb_mx_rows* q, int32_t transpose,
+                                      int32_t out_dtype);
+TLB_API int tlb_mx_grad(const void* g, int32_t g_dtype, int64_t m, int32_t n, const tlb_mx_rows* q, int32_t transpose,
+                        void* out, int32_t out_dtype, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ---- introspection ---------------------------------------------------------------------
  * Launch geometry the fused kernel would use for `desc` (for tests and the

@@ -19,6 +19,21 @@ from .augment import pick_crops
 from .sharding import (CONTIGUOUS, HASH_BASED, INTERLEAVED, DistributedSampler, ShardingCoordinator,
                        ShardingStrategy, direct_order, shard_indices)
 
+# Resolved on first use: these subclass or hold torch types, and importing the package does not import torch.
+_WITH_TORCH = {"MxTensor": "mx", "MxCache": "mx", "mx_quantize": "mx", "mx_dequantize": "mx", "mx_matmul": "mx",
+               "mx_linear": "mx", "CudaFeatureLoader": "feature_loader"}
+
+
+def __getattr__(name):
+    if name in _WITH_TORCH:
+        from importlib import import_module
+
+        value = getattr(import_module("." + _WITH_TORCH[name], __name__), name)
+        globals()[name] = value
+        return value
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
+
 __version__ = "0.1.0"
 __all__ = [
     "IMAGENET_MEAN", "IMAGENET_STD", "cuda_available", "cuda_device_name", "cuda_resize_normalize",
@@ -26,6 +41,7 @@ __all__ = [
     "cuda_resize_normalize_from_device",
     "fused_transform", "fused_plan", "make_desc", "features", "launch_count", "cuda_video_yuv420_batch", "cuda_video_clip_yuv420", "video_yuv420",
     "CudaResidentLoader", "CudaStreamLoader", "_CudaArray",
+    "MxTensor", "MxCache", "mx_quantize", "mx_dequantize", "mx_matmul", "mx_linear", "CudaFeatureLoader",
     "DataLoader", "DirectBatchLoader", "ImageNetNormalize", "pick_crops",
     "ShardingStrategy", "ShardingCoordinator", "DistributedSampler", "direct_order", "shard_indices",
     "CONTIGUOUS", "INTERLEAVED", "HASH_BASED",

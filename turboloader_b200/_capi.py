@@ -13,12 +13,40 @@ from . import build as _build
 TLB_OK = 0
 ERR_NAMES = {1: "INVALID_ARG", 2: "BAD_BOX", 3: "BAD_INDEX", 4: "TOO_WIDE", 5: "CUDA", 6: "NO_DEVICE",
              7: "TOO_LARGE"}
-TLB_F32, TLB_BF16 = 0, 1
+TLB_F32, TLB_BF16, TLB_F16 = 0, 1, 2
 TLB_NCHW, TLB_NHWC = 0, 1
 STATIC_SCRATCH_BYTES = 32 * 1024 * 1024  # TLB_STATIC_SCRATCH_BYTES
 STATIC_MAX_SAMPLES = 4096                # TLB_STATIC_MAX_SAMPLES
-DEV_BAD_INDEX, DEV_BAD_BOX, DEV_TOO_WIDE, DEV_COPY_TIMEOUT = 1, 2, 4, 8
+DEV_BAD_INDEX, DEV_BAD_BOX, DEV_TOO_WIDE, DEV_COPY_TIMEOUT, DEV_BAD_LENGTH = 1, 2, 4, 8, 16
 FLAG_LAUNCH_OVERLAP = 1                  # TLB_FLAG_LAUNCH_OVERLAP
+
+
+MX_MAX_COLS = 1 << 20                    # TLB_MX_MAX_COLS
+MX_SCAN_SAMPLES = 256                    # TLB_MX_SCAN_SAMPLES
+
+
+class MxRows(C.Structure):
+    """``tlb_mx_rows`` (field order and types must match the header)."""
+    _fields_ = [
+        ("codes", C.c_void_p),
+        ("scales", C.c_void_p),
+        ("rows", C.c_int64),
+        ("cols", C.c_int32),
+        ("format", C.c_int32),
+        ("scale", C.c_float),
+        ("scale_dev", C.c_void_p),
+    ]
+
+
+class MxCache(C.Structure):
+    """``tlb_mx_cache`` (field order and types must match the header)."""
+    _fields_ = [
+        ("rows", MxRows),
+        ("tokens", C.c_int32),
+        ("lengths", C.c_void_p),
+        ("owner", C.c_void_p),
+        ("status", C.c_void_p),
+    ]
 
 
 class TransformDesc(C.Structure):
@@ -174,6 +202,20 @@ def load() -> C.CDLL:
     lib.tlb_fused_plan.restype = C.c_int
     lib.tlb_fused_plan.argtypes = [C.POINTER(TransformDesc)] + [C.POINTER(C.c_int32)] * 5
     lib.tlb_launch_count.restype = C.c_uint64
+    rows, cache, i32, i64, ptr = C.POINTER(MxRows), C.POINTER(MxCache), C.c_int32, C.c_int64, C.c_void_p
+    for name, result, args in (
+            ("tlb_mx_code_pitch", i64, [i32, i32]),
+            ("tlb_mx_scale_pitch", i64, [i32, i32]),
+            ("tlb_mx_quantize", C.c_int, [rows, ptr, i32, i64, ptr]),
+            ("tlb_mx_write", C.c_int, [cache, ptr, i64, ptr, i32, i64, i64, ptr, ptr]),
+            ("tlb_mx_read", C.c_int, [cache, ptr, i64, ptr, i32, ptr, ptr]),
+            ("tlb_mx_read_codes", C.c_int, [cache, ptr, i64, ptr, ptr, ptr, ptr]),
+            ("tlb_mx_matmul_workspace", i64, [rows, rows, i32]),
+            ("tlb_mx_matmul", C.c_int, [rows, rows, ptr, i32, ptr, i64, ptr]),
+            ("tlb_mx_grad_workspace", i64, [i32, i64, i32, rows, i32, i32]),
+            ("tlb_mx_grad", C.c_int, [ptr, i32, i64, i32, rows, i32, ptr, i32, ptr, i64, ptr])):
+        fn = getattr(lib, name)
+        fn.restype, fn.argtypes = result, args
     i64p = C.POINTER(C.c_int64)
     lib.tlb_shard_indices.restype = C.c_int64
     lib.tlb_shard_indices.argtypes = [C.c_int32, C.c_int64, C.c_int64, C.c_int64, i64p, C.c_int64]

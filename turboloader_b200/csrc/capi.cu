@@ -23,6 +23,7 @@
 #include "video_params.h"
 #include "antialias_params.h"
 #include "host_gather.h"
+#include "mx_params.h"
 
 namespace {
 
@@ -42,6 +43,14 @@ int fail(int code, const char* fmt, ...) {
 int cuda_fail(cudaError_t e, const char* what) {
     return fail(TLB_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
+
+}  // namespace
+
+namespace tlb {
+int report(int code, const char* message) { return fail(code, "%s", message); }
+}  // namespace tlb
+
+namespace {
 
 #define TLB_CUDA(call)                                      \
     do {                                                    \
@@ -1096,7 +1105,7 @@ int tlb_fused_plan(const tlb_transform_desc* desc, int32_t* grid, int32_t* block
 
 uint64_t tlb_launch_count(void) {
     return tlb::launch_count() + tlb::video_launch_count() + tlb::antialias_launch_count() + tlb::normalize_copy_launch_count() +
-           g_extra_launches.load(std::memory_order_relaxed);
+           tlb::mx_launch_count() + g_extra_launches.load(std::memory_order_relaxed);
 }
 
 }  // extern "C"

@@ -1,0 +1,80 @@
+// Launch parameters of the microscaled operators (mx_rows.cu, mx_matmul.cu, mx_grad.cu), shared with
+// their host C ABI (mx_capi.cu).
+#pragma once
+#include <cuda_runtime.h>
+
+namespace tlb {
+
+enum MxFormat { kNvfp4 = 0, kMxfp4 = 1, kMxfp8 = 2 };
+enum MxDtype { kF32 = 0, kBf16 = 1, kF16 = 2 };
+
+// Rows are padded to 128 values, with zero codes and zero scale bytes, so that every row of codes
+// starts on a 64-byte boundary and every row of scales on a 4-byte one.
+constexpr int kMxPad = 128;
+__host__ __device__ inline int mx_padded(int cols) { return (cols + kMxPad - 1) / kMxPad * kMxPad; }
+__host__ __device__ inline int mx_block(int format) { return format == kNvfp4 ? 16 : 32; }
+__host__ __device__ inline int mx_code_pitch(int format, int cols) { return format == kMxfp8 ? mx_padded(cols) : mx_padded(cols) / 2; }
+__host__ __device__ inline int mx_scale_pitch(int format, int cols) { return mx_padded(cols) / mx_block(format); }
+
+struct MxRows {
+    unsigned char* codes;
+    unsigned char* scales;
+    long long rows;
+    int cols, format;
+    float scale;             // tensor scale = scale * (scale_dev ? *scale_dev : 1)
+    const float* scale_dev;
+};
+
+// Rows of `n` samples of `tokens` rows each, quantised into or read from the slots of a cache.
+struct MxMove {
+    MxRows q;                // the cache (or a plain matrix: tokens = 1, index = nullptr)
+    long long slots;         // samples the cache holds
+    int tokens;              // rows per sample
+    long long n;             // samples of this call
+    const long long* index;  // slot of every sample, nullptr: slot i = i
+    int* cache_lengths;      // rows in use per slot, or nullptr: all
+    const int* lengths;      // write: rows of every sample, or nullptr: all
+    int* lengths_out;        // read: rows in use of every sample, or nullptr
+    int* owner;              // write: [slots] words, -1 between calls (see mx_rows.cu)
+    int use_owner;           // write: 1 = duplicates were resolved in `owner`, 0 = look for them in `index`
+    unsigned* status;
+    const void* in;          // write: values, row pitch and sample pitch in elements
+    long long row_pitch, sample_pitch;
+    void* out;               // read: values, packed
+    unsigned char* out_codes;   // read of codes: both packed
+    unsigned char* out_scales;
+    int dtype;
+};
+
+int launch_mx_write(const MxMove& p, void* stream);       // returns a cudaError_t value
+int launch_mx_read(const MxMove& p, void* stream);
+int launch_mx_read_codes(const MxMove& p, void* stream);
+
+struct MxProduct {
+    MxRows a, b;             // (m, k) and (n, k)
+    void* out;               // (m, n) packed
+    int out_dtype;
+    void* workspace;
+};
+size_t mx_matmul_workspace(const MxProduct& p);
+int launch_mx_matmul(const MxProduct& p, void* stream);
+
+// out = alpha * op(g) * values(q): op(g) = g (m, n) with q of n rows, or its transpose with q of m rows.
+struct MxGrad {
+    const void* g;           // (m, n) packed
+    int g_dtype;
+    long long m;
+    int n;
+    int transpose;           // 0: out (m, cols), sums over n.  1: out (n, cols), sums over m
+    MxRows q;
+    void* out;
+    int out_dtype;
+    void* workspace;
+};
+size_t mx_grad_workspace(const MxGrad& p);
+int launch_mx_grad(const MxGrad& p, void* stream);
+
+unsigned long long mx_launch_count();
+void mx_count_launch();
+
+}  // namespace tlb

@@ -1,0 +1,462 @@
+"""Microscaled rows: quantisation of features to 4 or 8 bits, a cache that holds them, and the products on them.
+
+A feature set -- the token outputs of a frozen image encoder -- is many times larger than the images it came
+from.  Here it stays resident in HBM at 4.5 (``nvfp4``), 4.25 (``mxfp4``) or 8.25 (``mxfp8``) bits a value, is
+written sample by sample, served in shuffled order, and goes through the next model's first linear layer without
+being widened first.  The formats, the layout of the rows and the rules for special values stand in
+``include/turboloader_b200.h`` ("microscaled rows").  torch allocates memory and names the current stream; every
+computation happens inside the C-ABI library, on the current stream (or ``stream``), without synchronisation, so
+all of it can be captured into CUDA graphs.
+
+No counterpart in the reference, whose resident loader keeps uint8 pixels (turboloader/cuda_loader.py:385-535).
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes as C
+
+import torch
+
+from . import _capi
+
+__all__ = ["MxTensor", "MxCache", "mx_quantize", "mx_dequantize", "mx_matmul", "mx_linear"]
+
+_FORMATS = {"nvfp4": 0, "mxfp4": 1, "mxfp8": 2}
+_BLOCK = (16, 32, 32)
+_DTYPES = {torch.float32: _capi.TLB_F32, torch.bfloat16: _capi.TLB_BF16, torch.float16: _capi.TLB_F16}
+
+
+def _format_id(format):
+    try:
+        return _FORMATS[format]
+    except (KeyError, TypeError):
+        raise ValueError(f"format must be one of {tuple(_FORMATS)}, got {format!r}") from None
+
+
+def _dtype_id(dtype, what):
+    try:
+        return _DTYPES[dtype]
+    except KeyError:
+        raise TypeError(f"{what} must be float32, bfloat16 or float16, got {dtype}") from None
+
+
+def _pitches(fmt, cols):
+    if not 1 <= cols <= _capi.MX_MAX_COLS:
+        raise ValueError(f"rows must have between 1 and {_capi.MX_MAX_COLS} values, got {cols}")
+    padded = (cols + 127) // 128 * 128
+    return (padded if fmt == 2 else padded // 2), padded // _BLOCK[fmt]
+
+
+def _cuda(t, what):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError(f"{what} must be a CUDA tensor")
+    return t
+
+
+def _table(t, dtype, n, device, what):
+    """A contiguous 1-D device table of ``n`` entries."""
+    _cuda(t, what)
+    if t.dtype != dtype or t.dim() != 1 or not t.is_contiguous():
+        raise TypeError(f"{what} must be a contiguous 1-D {dtype} tensor")
+    if n is not None and t.shape[0] != n:
+        raise ValueError(f"{what} must have {n} entries, got {t.shape[0]}")
+    if t.device != device:
+        raise ValueError(f"{what} is on {t.device}, not on {device}")
+    return t
+
+
+def _check_scale(scale, device):
+    if isinstance(scale, torch.Tensor):
+        if scale.device != device or scale.dtype != torch.float32 or scale.numel() != 1:
+            raise TypeError(f"a scale tensor must be one float32 value on {device}")
+        return scale.detach()
+    scale = float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError("scale must be positive and finite")
+    return scale
+
+
+@contextlib.contextmanager
+def _elsewhere(device, stream):
+    with torch.cuda.device(device):
+        if stream is None:
+            yield torch.cuda.current_stream(device).cuda_stream
+        else:
+            with torch.cuda.stream(stream):  # outputs and workspaces belong to the stream that uses them
+                yield stream.cuda_stream
+
+
+class _Here:
+    """The usual case of ``_on``: the tensors' device is the current one, and no stream is named."""
+    __slots__ = ("handle",)
+
+    def __init__(self, handle):
+        self.handle = handle
+
+    def __enter__(self):
+        return self.handle
+
+    def __exit__(self, *exc):
+        return False
+
+
+def _on(device, stream):
+    """Context in which the library is called for tensors of ``device``: gives the raw stream."""
+    if stream is None and torch.cuda.current_device() == device.index:
+        return _Here(torch.cuda.current_stream().cuda_stream)
+    if stream is not None and stream.device != device:
+        raise ValueError(f"stream is on {stream.device}, the tensors on {device}")
+    return _elsewhere(device, stream)
+
+
+def _rows_struct(codes, scales, rows, cols, fmt, scale):
+    if isinstance(scale, torch.Tensor):
+        return _capi.MxRows(codes.data_ptr(), scales.data_ptr(), rows, cols, fmt, 1.0, scale.data_ptr())
+    return _capi.MxRows(codes.data_ptr(), scales.data_ptr(), rows, cols, fmt, scale, None)
+
+
+def _check_held(codes, scales, rows, cols, fmt):
+    """codes (..., code pitch) and scales (..., scale pitch): uint8, contiguous, `rows` rows in all."""
+    cp, sp = _pitches(fmt, cols)
+    for t, pitch, what in ((codes, cp, "codes"), (scales, sp, "scales")):
+        _cuda(t, what)
+        if t.dtype != torch.uint8 or not t.is_contiguous() or t.dim() < 1 or t.shape[-1] != pitch:
+            raise ValueError(f"{what} must be a contiguous uint8 tensor with rows of {pitch} bytes")
+        if t.numel() != rows * pitch:
+            raise ValueError(f"{what} must hold {rows} rows, got {t.numel() // pitch}")
+    if codes.device != scales.device:
+        raise ValueError(f"codes are on {codes.device}, scales on {scales.device}")
+    if codes.data_ptr() % 16 or scales.data_ptr() % 4:
+        raise ValueError("codes must be 16-byte and scales 4-byte aligned")
+
+
+class MxTensor:
+    """Microscaled rows: ``codes`` and ``scales`` (uint8 CUDA tensors, rows padded to 128 values as the C header
+    says) standing for values of ``shape`` (the last dimension is the rows' length), times ``scale`` -- a float,
+    or one float32 value on the device.  Holds the tensors it is given, without a copy."""
+
+    __slots__ = ("codes", "scales", "shape", "format", "scale", "_fmt", "_rows")
+
+    def __init__(self, codes, scales, shape, format, *, scale=1.0):
+        self._fmt = _format_id(format)
+        shape = tuple(int(s) for s in shape)
+        if not shape:
+            raise ValueError("an MxTensor has at least one dimension")
+        self._rows = 1
+        for s in shape[:-1]:
+            self._rows *= s
+        _check_held(codes, scales, self._rows, shape[-1], self._fmt)
+        self.codes, self.scales, self.shape, self.format = codes, scales, shape, format
+        self.scale = 1.0 if scale == 1.0 and not isinstance(scale, torch.Tensor) else _check_scale(scale, codes.device)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def _struct(self):
+        return _rows_struct(self.codes, self.scales, self._rows, self.shape[-1], self._fmt, self.scale)
+
+    def dequantize(self, dtype=torch.float32):
+        return mx_dequantize(self, dtype)
+
+    def __repr__(self):
+        return f"MxTensor(shape={self.shape}, format={self.format!r}, device={self.device})"
+
+
+def _as_rows(x, what):
+    """(data, rows, cols, row pitch) of (..., cols) values whose rows lie at equal distances."""
+    _cuda(x, what)
+    if x.dim() < 1:
+        raise ValueError(f"{what} must have at least one dimension")
+    cols = x.shape[-1]
+    if x.stride(-1) != 1 and cols != 1:
+        raise ValueError(f"the values of a row of {what} must be contiguous")
+    if x.dim() == 2:
+        rows, pitch = x.shape[0], x.stride(0)
+    elif x.dim() == 1:
+        rows, pitch = 1, cols
+    else:
+        try:
+            flat = x.detach().view(-1, cols) if x.numel() else x.detach().reshape(-1, cols)
+        except RuntimeError:
+            raise ValueError(f"the rows of {what} must lie at equal distances") from None
+        rows, pitch = flat.shape[0], flat.stride(0)
+    if rows > 1 and pitch < cols:
+        raise ValueError(f"the rows of {what} overlap (pitch {pitch}, {cols} values)")
+    return rows, cols, pitch
+
+
+def mx_quantize(x, format="nvfp4", *, scale=1.0, stream=None):
+    """``x`` (..., cols), float32, bfloat16 or float16, as an ``MxTensor``.  The values of a row must be
+    contiguous and the rows equally spaced (a slice of a wider matrix will do).  ``scale``: the tensor scale
+    that values are divided by first, a float or one float32 value on the device; a power of two loses
+    nothing.  For ``nvfp4``, ``max|x| / 2688`` rounded up to a power of two uses the range of its scales."""
+    fmt = _format_id(format)
+    rows, cols, pitch = _as_rows(x, "x")
+    dt = _dtype_id(x.dtype, "x")
+    cp, sp = _pitches(fmt, cols)
+    device = x.device
+    scale = _check_scale(scale, device)
+    with _on(device, stream) as handle:
+        codes = torch.empty((rows, cp), dtype=torch.uint8, device=device)
+        scales = torch.empty((rows, sp), dtype=torch.uint8, device=device)
+        q = MxTensor(codes, scales, x.shape, format, scale=scale)
+        _capi.check(_capi.load().tlb_mx_quantize(C.byref(q._struct()), x.data_ptr(), dt, pitch, handle))
+    return q
+
+
+def _out(out, shape, dtype, device):
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    _cuda(out, "out")
+    if out.dtype != dtype or tuple(out.shape) != tuple(shape) or not out.is_contiguous() or out.device != device:
+        raise ValueError(f"out must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}")
+    if out.data_ptr() % 16:
+        raise ValueError("out must be 16-byte aligned")
+    return out
+
+
+def mx_dequantize(q, dtype=torch.float32, *, out=None, stream=None):
+    """The values that ``q`` stands for: code * block scale * tensor scale in fp32, rounded once to ``dtype``."""
+    dt = _dtype_id(dtype, "dtype")
+    with _on(q.device, stream) as handle:
+        out = _out(out, q.shape, dtype, q.device)
+        cache = _capi.MxCache(q._struct(), 1, None, None, None)
+        _capi.check(_capi.load().tlb_mx_read(C.byref(cache), None, q._rows, out.data_ptr(), dt, None, handle))
+    return out
+
+
+def _check_pair(a, b):
+    if not isinstance(a, MxTensor) or not isinstance(b, MxTensor):
+        raise TypeError("a and b must be MxTensors")
+    if a._fmt != b._fmt:
+        raise ValueError(f"a is {a.format}, b is {b.format}")
+    if len(b.shape) != 2 or a.shape[-1] != b.shape[1]:
+        raise ValueError(f"shapes {a.shape} and {b.shape} do not multiply: b must be (n, {a.shape[-1]})")
+    if a.device != b.device:
+        raise ValueError(f"a is on {a.device}, b on {b.device}")
+
+
+def _workspace(size, device):
+    return torch.empty(size, dtype=torch.uint8, device=device) if size > 0 else None
+
+
+def mx_matmul(a, b, dtype=torch.bfloat16, *, out=None, stream=None):
+    """``a`` (..., k) times the transpose of ``b`` (n, k), two ``MxTensor`` of one format: (..., n) of ``dtype``.
+    The products of the codes enter whole and are summed in fp32; the result is rounded once."""
+    _check_pair(a, b)
+    dt = _dtype_id(dtype, "dtype")
+    lib = _capi.load()
+    device = a.device
+    with _on(device, stream) as handle:
+        out = _out(out, (*a.shape[:-1], b.shape[0]), dtype, device)
+        sa, sb = a._struct(), b._struct()
+        size = lib.tlb_mx_matmul_workspace(C.byref(sa), C.byref(sb), dt)
+        ws = _workspace(size, device)
+        _capi.check(lib.tlb_mx_matmul(C.byref(sa), C.byref(sb), out.data_ptr(), dt, ws.data_ptr() if ws is not None else None,
+                                      size, handle))
+    return out
+
+
+def _grad(g, q, transpose, dtype):
+    """g (m, n) times values(q) (n, k), or with ``transpose`` g^T times values(q) (m, k); in ``dtype``."""
+    lib = _capi.load()
+    device = g.device
+    m, n = g.shape
+    dt, gt = _DTYPES[dtype], _DTYPES[g.dtype]
+    with _on(device, None) as handle:
+        out = torch.empty((n if transpose else m, q.shape[-1]), dtype=dtype, device=device)
+        sq = q._struct()
+        size = lib.tlb_mx_grad_workspace(gt, m, n, C.byref(sq), transpose, dt)
+        ws = _workspace(size, device)
+        _capi.check(lib.tlb_mx_grad(g.data_ptr(), gt, m, n, C.byref(sq), transpose, out.data_ptr(), dt,
+                                    ws.data_ptr() if ws is not None else None, size, handle))
+    return out
+
+
+def _spaced(x):
+    """``x`` as rows that mx_quantize takes; a copy only where its strides demand one."""
+    x = x.detach()
+    try:
+        _as_rows(x, "x")
+        return x
+    except ValueError:
+        return x.contiguous()
+
+
+class _MxLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, held_x, held_w, format, scale, weight_scale, dtype):
+        qx = held_x if x is None else mx_quantize(_spaced(x), format, scale=scale)
+        qw = held_w if weight is None else mx_quantize(_spaced(weight), format, scale=weight_scale)
+        y = mx_matmul(qx, qw, dtype)
+        ctx.x_dtype = None if x is None else x.dtype
+        ctx.w_dtype = None if weight is None else weight.dtype
+        keep_x, keep_w = weight is not None and ctx.needs_input_grad[1], x is not None and ctx.needs_input_grad[0]
+        ctx.held = [(q.shape, q.format, q.scale) if keep else None for q, keep in ((qx, keep_x), (qw, keep_w))]
+        ctx.x_shape = qx.shape
+        ctx.save_for_backward(*([qx.codes, qx.scales] if keep_x else []), *([qw.codes, qw.scales] if keep_w else []))
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        saved = list(ctx.saved_tensors)
+        kept = []
+        for held in ctx.held:
+            kept.append(None if held is None else MxTensor(saved.pop(0), saved.pop(0), held[0], held[1], scale=held[2]))
+        qx, qw = kept
+        g = g.reshape(-1, g.shape[-1]).contiguous()
+        if g.data_ptr() % 16:
+            g = g.clone()
+        gx = _grad(g, qw, 0, ctx.x_dtype).view(ctx.x_shape) if qw is not None else None
+        gw = _grad(g, qx, 1, ctx.w_dtype) if qx is not None else None
+        return gx, gw, None, None, None, None, None, None
+
+
+def mx_linear(x, weight, format="nvfp4", *, scale=1.0, weight_scale=1.0, dtype=None):
+    """``x @ weight.T`` on microscaled operands, differentiable: (..., k), (n, k) -> (..., n) of ``dtype``.
+
+    ``x`` and ``weight`` are float tensors, quantised to ``format`` by this call (``scale`` and ``weight_scale``
+    are their tensor scales), or ``MxTensor`` of that format, used as they are (cached features, a frozen weight).
+    Gradients flow to the float tensors, straight through their quantisation: ``dx = g @ values(weight)`` and
+    ``dweight = g.T @ values(x)``, with every value of g entering whole, sums in fp32, in the operand's own type;
+    for the backward pass only the codes are kept.  An ``MxTensor`` must stay unchanged until then.  ``dtype``
+    (the result's): by default ``weight``'s, else ``x``'s, else bfloat16."""
+    _format_id(format)
+    held_x, held_w = (t if isinstance(t, MxTensor) else None for t in (x, weight))
+    for t, what in ((x, "x"), (weight, "weight")):
+        if isinstance(t, MxTensor):
+            if t.format != format:
+                raise ValueError(f"{what} is {t.format}, not {format}")
+        else:
+            _dtype_id(_cuda(t, what).dtype, what)
+            if t.dim() < 1:
+                raise ValueError(f"{what} must have at least one dimension")
+    if len(weight.shape) != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"shapes {tuple(x.shape)} and {tuple(weight.shape)} do not multiply: weight must be (n, {x.shape[-1]})")
+    if x.device != weight.device:
+        raise ValueError(f"x is on {x.device}, weight on {weight.device}")
+    if dtype is None:
+        dtype = weight.dtype if held_w is None else x.dtype if held_x is None else torch.bfloat16
+    _dtype_id(dtype, "dtype")
+    return _MxLinear.apply(None if held_x is not None else x, None if held_w is not None else weight, held_x, held_w,
+                           format, scale, weight_scale, dtype)
+
+
+class MxCache:
+    """Samples of ``tokens`` rows of ``cols`` values, held as microscaled rows: ``codes`` (slots, tokens, code
+    pitch) and ``scales`` (slots, tokens, scale pitch), and for samples of different lengths ``lengths`` (slots,)
+    int32.  Wraps the tensors it is given; ``MxCache.empty`` makes them.
+
+    ``status``: one int32 value on the device that the kernels OR their TLB_DEV_* bits into (``empty`` gives one)."""
+
+    def __init__(self, codes, scales, cols, format, *, lengths=None, scale=1.0, status=None):
+        self._fmt = _format_id(format)
+        _cuda(codes, "codes")
+        if codes.dim() != 3:
+            raise ValueError("codes must be (slots, tokens, code pitch)")
+        self.slots, self.tokens, self.cols, self.format = int(codes.shape[0]), int(codes.shape[1]), int(cols), format
+        if self.tokens < 1:
+            raise ValueError("a cache needs at least one row a sample")
+        _check_held(codes, scales, self.slots * self.tokens, self.cols, self._fmt)
+        self.codes, self.scales = codes, scales
+        self.lengths = None if lengths is None else _table(lengths, torch.int32, self.slots, codes.device, "lengths")
+        self.scale = _check_scale(scale, codes.device)
+        self.status = None if status is None else _table(status, torch.int32, 1, codes.device, "status")
+        self._owner = None
+
+    @classmethod
+    def empty(cls, slots, tokens, cols, format="nvfp4", *, ragged=False, scale=1.0, device=None):
+        """A cache of zero rows (``ragged``: of samples of length zero)."""
+        device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        cp, sp = _pitches(_format_id(format), int(cols))
+        return cls(torch.zeros((int(slots), int(tokens), cp), dtype=torch.uint8, device=device),
+                   torch.zeros((int(slots), int(tokens), sp), dtype=torch.uint8, device=device), cols, format,
+                   lengths=torch.zeros(int(slots), dtype=torch.int32, device=device) if ragged else None, scale=scale,
+                   status=torch.zeros(1, dtype=torch.int32, device=device))
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def device_status(self) -> int:
+        """Status bits the kernels OR-ed so far (synchronises); 0 when every index and length was valid."""
+        return 0 if self.status is None else int(self.status.item())
+
+    def _struct(self):
+        rows = _rows_struct(self.codes, self.scales, self.slots * self.tokens, self.cols, self._fmt, self.scale)
+        return _capi.MxCache(rows, self.tokens, None if self.lengths is None else self.lengths.data_ptr(),
+                             None if self._owner is None else self._owner.data_ptr(),
+                             None if self.status is None else self.status.data_ptr())
+
+    def write(self, index, x, *, lengths=None, stream=None):
+        """Quantises sample ``x[i]`` (tokens, cols) into slot ``index[i]`` (int64 CUDA tensor).  With ``lengths``
+        (int32, for a cache that has lengths) only the first ``lengths[i]`` rows are read and written; the slot's
+        other rows stay as they were.  Without, all rows are there.  A slot named twice takes the last of its
+        samples; an index outside the cache is skipped and reported in ``status``."""
+        device = self.device
+        _cuda(x, "x")
+        if x.dim() == 2 and self.tokens == 1:
+            x = x.unsqueeze(1)
+        if x.dim() != 3 or x.shape[1] != self.tokens or x.shape[2] != self.cols:
+            raise ValueError(f"x must be (n, {self.tokens}, {self.cols}), got {tuple(x.shape)}")
+        if x.device != device:
+            raise ValueError(f"x is on {x.device}, the cache on {device}")
+        n = x.shape[0]
+        dt = _dtype_id(x.dtype, "x")
+        _table(index, torch.int64, n, device, "index")
+        if lengths is not None:
+            if self.lengths is None:
+                raise ValueError("lengths given for a cache without lengths")
+            _table(lengths, torch.int32, n, device, "lengths")
+        if n == 0:
+            return
+        if x.stride(2) != 1 and self.cols != 1:
+            raise ValueError("the values of a row of x must be contiguous")
+        if (self.tokens > 1 and x.stride(1) < self.cols) or (n > 1 and x.stride(0) < self.cols):
+            raise ValueError("the rows of x overlap")
+        with _on(device, stream) as handle:
+            if self._owner is None and n > _capi.MX_SCAN_SAMPLES:
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError(f"write more than {_capi.MX_SCAN_SAMPLES} samples once before the capture: the first such call allocates")
+                self._owner = torch.full((self.slots,), -1, dtype=torch.int32, device=device)
+            _capi.check(_capi.load().tlb_mx_write(C.byref(self._struct()), index.data_ptr(), n, x.data_ptr(), dt,
+                                                  x.stride(1), x.stride(0), None if lengths is None else lengths.data_ptr(),
+                                                  handle))
+
+    def _picked(self, index):
+        if index is None:
+            return self.slots, None
+        _table(index, torch.int64, None, self.device, "index")
+        return index.shape[0], index.data_ptr()
+
+    def read(self, index=None, dtype=torch.bfloat16, *, out=None, stream=None):
+        """Samples ``index`` (int64 CUDA tensor; None: all, in order) as values (n, tokens, cols) of ``dtype``, zeros
+        behind a sample's length and for an index outside the cache (reported in ``status``).  A cache with
+        lengths gives ``(values, lengths)``."""
+        n, at = self._picked(index)
+        dt = _dtype_id(dtype, "dtype")
+        device = self.device
+        with _on(device, stream) as handle:
+            out = _out(out, (n, self.tokens, self.cols), dtype, device)
+            lengths = None if self.lengths is None else torch.empty(n, dtype=torch.int32, device=device)
+            _capi.check(_capi.load().tlb_mx_read(C.byref(self._struct()), at, n, out.data_ptr(), dt,
+                                                 None if lengths is None else lengths.data_ptr(), handle))
+        return out if lengths is None else (out, lengths)
+
+    def read_mx(self, index=None, *, stream=None):
+        """The same samples as they are held: an ``MxTensor`` (n, tokens, cols) with memory of its own, zero rows
+        where ``read`` gives zeros; with ``(…, lengths)`` for a cache that has them."""
+        n, at = self._picked(index)
+        device = self.device
+        with _on(device, stream) as handle:
+            codes = torch.empty((n, self.tokens, self.codes.shape[2]), dtype=torch.uint8, device=device)
+            scales = torch.empty((n, self.tokens, self.scales.shape[2]), dtype=torch.uint8, device=device)
+            lengths = None if self.lengths is None else torch.empty(n, dtype=torch.int32, device=device)
+            _capi.check(_capi.load().tlb_mx_read_codes(C.byref(self._struct()), at, n, codes.data_ptr(), scales.data_ptr(),
+                                                       None if lengths is None else lengths.data_ptr(), handle))
+        q = MxTensor(codes, scales, (n, self.tokens, self.cols), self.format, scale=self.scale)
+        return q if lengths is None else (q, lengths)
