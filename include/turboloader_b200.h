@@ -428,6 +428,11 @@ TLB_API int64_t tlb_mx_matmul_workspace(const tlb_mx_rows* a, const tlb_mx_rows*
 TLB_API int tlb_mx_matmul(const tlb_mx_rows* a, const tlb_mx_rows* b, void* out, int32_t out_dtype, void* workspace,
                           int64_t workspace_bytes, void* stream);
 
+/* Products and gradients on the current device since the library was loaded whose kernels gave up a
+ * bounded wait (seconds without progress) and left their result incomplete: 0 in a healthy process.
+ * Synchronises. */
+TLB_API int tlb_mx_incomplete(uint32_t* count);
+
 /* Gradients of that product with respect to the values of an operand, g (m, n) packed:
  *   transpose = 0: out (m, q.cols) = g * values(q),    q = b (n rows): the gradient of a
  *   transpose = 1: out (n, q.cols) = g^T * values(q),  q = a (m rows): the gradient of b

@@ -21,7 +21,7 @@ from .sharding import (CONTIGUOUS, HASH_BASED, INTERLEAVED, DistributedSampler, 
 
 # Resolved on first use: these subclass or hold torch types, and importing the package does not import torch.
 _WITH_TORCH = {"MxTensor": "mx", "MxCache": "mx", "mx_quantize": "mx", "mx_dequantize": "mx", "mx_matmul": "mx",
-               "mx_linear": "mx", "CudaFeatureLoader": "feature_loader"}
+               "mx_linear": "mx", "mx_incomplete": "mx", "CudaFeatureLoader": "feature_loader"}
 
 
 def __getattr__(name):
@@ -41,7 +41,7 @@ __all__ = [
     "cuda_resize_normalize_from_device",
     "fused_transform", "fused_plan", "make_desc", "features", "launch_count", "cuda_video_yuv420_batch", "cuda_video_clip_yuv420", "video_yuv420",
     "CudaResidentLoader", "CudaStreamLoader", "_CudaArray",
-    "MxTensor", "MxCache", "mx_quantize", "mx_dequantize", "mx_matmul", "mx_linear", "CudaFeatureLoader",
+    "MxTensor", "MxCache", "mx_quantize", "mx_dequantize", "mx_matmul", "mx_linear", "mx_incomplete", "CudaFeatureLoader",
     "DataLoader", "DirectBatchLoader", "ImageNetNormalize", "pick_crops",
     "ShardingStrategy", "ShardingCoordinator", "DistributedSampler", "direct_order", "shard_indices",
     "CONTIGUOUS", "INTERLEAVED", "HASH_BASED",

@@ -249,6 +249,14 @@ int tlb_mx_matmul(const tlb_mx_rows* a, const tlb_mx_rows* b, void* out, int32_t
     return TLB_OK;
 }
 
+int tlb_mx_incomplete(uint32_t* count) {
+    if (!count) return fail(TLB_ERR_INVALID_ARG, "count is NULL");
+    *count = 0;
+    if (int rc = need_device()) return rc;
+    if (int e = tlb::mx_gave_up(count)) return cuda_fail(e, "mx_incomplete");
+    return TLB_OK;
+}
+
 int64_t tlb_mx_grad_workspace(int32_t g_dtype, int64_t m, int32_t n, const tlb_mx_rows* q, int32_t transpose, int32_t out_dtype) {
     if (check_grad(g_dtype, m, n, q, transpose, out_dtype)) return -1;
     return static_cast<int64_t>(tlb::mx_grad_workspace(grad_of(g_dtype, m, n, *q, transpose, out_dtype)));

@@ -1,18 +1,23 @@
 // Product of two matrices of microscaled rows: out[m][n] = tsA tsB sum_k (cA sA)(cB sB), fp32 sums.
 //
-// product_kernel: one persistent CTA per SM, output tiles of 128 x tile_n (tile_n <= 224, a multiple of
-// 16), the block-scaled tensor-core instructions reading codes from shared memory and scales from TMEM.
-//   warp 0     copies code tiles (128 bytes of every row a stage) into a ring of kStages stages
-//   warp 1     moves the stage's scales into TMEM and issues four instructions a stage
-//   warps 2-3  idle (they keep the roles below on whole groups of four warps)
-//   warps 4-7  turn finished accumulators into output rows, while the next tile is being summed
-//   warps 8-11 read the stage's scale bytes and lay them out as the instructions want them: of a group of
-//              128 rows and 4 scales, row r takes word (r % 32) * 4 + r / 32 of 512 bytes
+// arrange_kernel lays the scales of both out as the tensor cores take them: groups of 128 rows and 4
+// scales, 512 bytes each, row r at word (r % 32) * 4 + r / 32.
+//
+// product_kernel: a pair of CTAs (a cluster of 2) makes output tiles of 256 x tile_n, tile_n <= 224 a
+// multiple of 16; each CTA holds 128 rows of A, half of B's rows, and 128 rows of the result.  Per CTA:
+//   warp 0      copies a stage -- 128 bytes of codes of every row, and their scales -- into a ring
+//   warp 1      (leader) moves the stage's scales into TMEM and issues four instructions a stage
+//   warps 4-11  turn finished accumulators into output rows, while the next tile is being summed
 // TMEM: two accumulators of tile_n columns, then the stage's scales: 16 columns for A (4 a group), 32 for
 // B.  The moves into the scale columns and the products that read them are issued by one thread and run in
 // that order, so the scales need no second buffer.
+//
+// The pair exists because of shared memory: 4-bit products of 128 x 208 tiles read 10.8 kB an instruction
+// and their copies write as much, more than the 128 bytes a cycle that an SM has; a pair reads and writes
+// half of B (8192^3 nvfp4: 392 us -> 224).  Where all of a tile's A fits beside the ring (k_stages <=
+// kSlots: 1024 values a row of 4 bits, 512 of 8), it stays in shared memory while the pair walks along its
+// row of tiles, and only B is copied for each: less to copy, and the result is written row after row.
 #include <atomic>
-#include <mutex>
 
 #include "mx_device.cuh"
 #include "mx_tma.cuh"
@@ -20,26 +25,56 @@
 namespace tlb {
 namespace {
 
-constexpr int kTileM = 128, kMaxTileN = 224;
-constexpr int kStages = 4;
-constexpr int kStageA = kTileM * 128, kStageB = kMaxTileN * 128, kScaleA = 2048, kScaleB = 4096;
-constexpr int kStageBytes = kStageA + kStageB + kScaleA + kScaleB;
-constexpr int kStagingPitch = 144, kStaging = 32 * kStagingPitch;  // an epilogue warp's 32 rows of 128 bytes
-constexpr int kSmem = 1024 + kStages * kStageBytes + 4 * kStaging + 256;
+constexpr int kTileM = 128, kMaxTileN = 224;  // rows of a CTA, columns of the pair
+constexpr int kCodesA = kTileM * 128, kCodesB = kMaxTileN / 2 * 128, kScaleA = 2048, kScaleB = 4096;
+// The same shared memory either way: whole stages, or slots that keep A and a longer ring for B.
+constexpr int kStages = 5, kStageBytes = kCodesA + kScaleA + kCodesB + kScaleB;
+constexpr int kSlots = 4, kSlotBytes = kCodesA + kScaleA, kStagesB = 6, kStageBBytes = kCodesB + kScaleB;
+constexpr int kRing = kSlots * kSlotBytes + kStagesB * kStageBBytes;
+static_assert(kStages * kStageBytes <= kRing && kStageBytes % 1024 == 0 && kSlotBytes % 1024 == 0 && kStageBBytes % 1024 == 0, "layout");
+constexpr int kStaging = 32 * 128;  // an epilogue warp's 32 rows of 128 bytes
+constexpr int kSmem = 1024 + kRing + 8 * kStaging;
 constexpr int kThreads = 384;
-static_assert(kSmem <= 227 * 1024, "shared memory");
+static_assert(kSmem <= 227 * 1024 - 512, "shared memory");
 constexpr unsigned kTmemColumns = 512, kTmemScaleA = 2 * kMaxTileN, kTmemScaleB = kTmemScaleA + 16;
 
 struct TileParams {
-    CUtensorMap map_a, map_b;
+    CUtensorMap map_a, map_b, map_sa, map_sb, map_out;
     MxProduct p;
-    int tile_n, n_tiles;
-    long long tiles;
+    int tile_n, n_tiles, groups_n;  // groups_n: groups of 128 rows that a tile's B scales take (1 or 2)
+    long long m_tiles, tiles;
     int k_stages;
-    int vec_ok;
+    int resident;  // A stays in shared memory over consecutive tiles of one row
+    int vec_ok;    // output rows are multiples of 16 bytes: written by tensor-map copies
 };
 
-// Scale words (4 scales) of a row in one stage, and instructions' share of them.
+// The tiles of a pair, row by row.  resident: a contiguous run, else every pairs-th.
+struct Walk {
+    long long tile, end, step;
+    __device__ explicit Walk(const TileParams& tp) {
+        const long long pair = blockIdx.x / 2, pairs = gridDim.x / 2;
+        tile = tp.resident ? tp.tiles * pair / pairs : pair;
+        end = tp.resident ? tp.tiles * (pair + 1) / pairs : tp.tiles;
+        step = tp.resident ? 1 : pairs;
+    }
+    __device__ void place(const TileParams& tp, int& m, int& n) const {
+        m = static_cast<int>(tile / tp.n_tiles);
+        n = static_cast<int>(tile - static_cast<long long>(m) * tp.n_tiles);
+    }
+};
+
+// A ring position and its parity.
+struct Ring {
+    unsigned s = 0, parity = 0;
+    __device__ void next(unsigned stages) {
+        if (++s == stages) s = 0, parity ^= 1u;
+    }
+};
+
+// Products that gave up a wait on this device since the library was loaded (their output is incomplete).
+__device__ unsigned g_gave_up;
+
+// Scale words (4 scales) of a row in one stage.
 template <int FMT> constexpr int kWords = FMT == kNvfp4 ? 4 : FMT == kMxfp4 ? 2 : 1;
 
 template <int FMT>
@@ -47,143 +82,218 @@ __device__ __forceinline__ void mma(unsigned d, unsigned long long a, unsigned l
     if (FMT == kNvfp4)
         asm volatile(
             "{ .reg .pred p;\n setp.ne.u32 p, %6, 0;\n"
-            "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d),
+            "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d),
             "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(more)
             : "memory");
     else if (FMT == kMxfp4)
         asm volatile(
             "{ .reg .pred p;\n setp.ne.u32 p, %6, 0;\n"
-            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d), "l"(a),
+            "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d), "l"(a),
             "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(more)
             : "memory");
     else
         asm volatile(
             "{ .reg .pred p;\n setp.ne.u32 p, %6, 0;\n"
-            "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d),
+            "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d),
             "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(more)
             : "memory");
 }
 
-// 32 rows of 16 bytes -> 4 TMEM columns, for each of the four groups of 32 lanes
+// 32 rows of 16 bytes -> 4 TMEM columns, for each of the four groups of 32 lanes, in both CTAs from their own memory
 __device__ __forceinline__ void copy_scales(unsigned tmem, unsigned smem) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(smem_desc(smem, 0, 128, 0)) : "memory");
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(smem_desc(smem, 0, 128, 0)) : "memory");
 }
 
-// The scale words of `row` in stage kt: zero behind the row's end and for rows behind the last.
-template <int FMT>
-__device__ __forceinline__ void load_scales(const MxRows& q, long long row, int kt, unsigned w[4]) {
-    constexpr int words = kWords<FMT>;
-    const int pitch = mx_scale_pitch(FMT, q.cols), at = kt * words * 4;
-    w[0] = w[1] = w[2] = w[3] = 0u;
-    if (row >= q.rows) return;
-    const unsigned char* s = q.scales + row * pitch + at;
-    if (FMT == kNvfp4) {  // the pitch is a multiple of 8
-        const uint2 lo = __ldg(reinterpret_cast<const uint2*>(s));
-        w[0] = lo.x, w[1] = lo.y;
-        if (at + 8 < pitch) {
-            const uint2 hi = __ldg(reinterpret_cast<const uint2*>(s) + 1);
-            w[2] = hi.x, w[3] = hi.y;
-        }
-    } else {
+// ---- scales ------------------------------------------------------------------------------------------------
+struct Arrange {
+    MxRows q;
+    unsigned* out;
+    int tile_rows;        // rows of a tile: 128 for A, tile_n for B
+    int groups;           // groups of 128 rows a tile takes
+    int words;            // words (4 scales) of a row, padded to whole stages
+    long long threads;    // tiles * groups * 32 * words / 4 (rounded up)
+};
+
+// A thread takes 4 rows (r, r + 32, ...) and up to 4 words of each: reads along the rows, writes 16 bytes a group.
+__device__ __forceinline__ void arrange(const Arrange& a, long long t) {
+    const int quads = (a.words + 3) / 4;
+    const int l = static_cast<int>(t % 32);
+    const long long rest = t / 32;
+    const int quad = static_cast<int>(rest % quads);
+    const long long tile_group = rest / quads;
+    const int group = static_cast<int>(tile_group % a.groups);
+    const long long tile = tile_group / a.groups;
+    const int pitch = mx_scale_pitch(a.q.format, a.q.cols) / 4;
+    unsigned w[4][4];
 #pragma unroll
-        for (int i = 0; i < words; ++i)
-            if (at + 4 * i < pitch) w[i] = __ldg(reinterpret_cast<const unsigned*>(s) + i);
+    for (int c = 0; c < 4; ++c) {
+        const int in_tile = group * 128 + c * 32 + l;
+        const long long row = tile * a.tile_rows + in_tile;
+        const bool there = in_tile < a.tile_rows && row < a.q.rows;
+        const unsigned* s = reinterpret_cast<const unsigned*>(a.q.scales) + (there ? row : 0) * pitch;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i][c] = there && quad * 4 + i < pitch ? __ldg(s + quad * 4 + i) : 0u;
     }
-}
-
-template <int FMT>
-__device__ __forceinline__ void store_scales(unsigned base, unsigned group_bytes, int row, const unsigned w[4]) {
-    const unsigned at = base + (row / 128) * 512 + (row % 32) * 16 + (row % 128) / 32 * 4;
 #pragma unroll
-    for (int i = 0; i < kWords<FMT>; ++i) asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + i * group_bytes), "r"(w[i]) : "memory");
+    for (int i = 0; i < 4; ++i)
+        if (quad * 4 + i < a.words)
+            reinterpret_cast<uint4*>(a.out)[((tile * a.words + quad * 4 + i) * a.groups + group) * 32 + l] = make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]);
 }
 
+__global__ void __launch_bounds__(256) arrange_kernel(Arrange a, Arrange b) {
+    let_next_start();
+    const long long t = blockIdx.x * 256ll + threadIdx.x;
+    if (t < a.threads) arrange(a, t);
+    else if (t - a.threads < b.threads) arrange(b, t - a.threads);
+}
+
+// ---- products ------------------------------------------------------------------------------------------------
 template <typename T, int FMT>
-__global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ TileParams tp) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ TileParams tp) {
     extern __shared__ unsigned char raw[];
-    __shared__ unsigned long long bars[4 * kStages + 4];
+    __shared__ unsigned long long bars[2 * kStagesB + 4 + 2 * kSlots];
     __shared__ unsigned tmem_base;
     __shared__ int gave_up;
     const unsigned smem = (smem_u32(raw) + 1023u) & ~1023u;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
+    const unsigned rank = __shfl_sync(0xffffffffu, cluster_rank(), 0);
     const MxProduct& p = tp.p;
     const int tile_n = tp.tile_n;
+    const unsigned ring = tp.resident ? kStagesB : kStages;
+    // Where A and its scales lie (of stage s, or of slot kt), and where stage s keeps B and its scales.
+    const unsigned a_base = smem, a_step = tp.resident ? kSlotBytes : kStageBytes;
+    const unsigned b_base = smem + (tp.resident ? kSlots * kSlotBytes : kCodesA + kScaleA), b_step = tp.resident ? kStageBBytes : kStageBytes;
 
-    const unsigned codes_full = smem_u32(bars), scales_full = codes_full + 8 * kStages, empty = scales_full + 8 * kStages;
-    const unsigned acc_full = empty + 8 * kStages, acc_empty = acc_full + 16;
+    const unsigned full = smem_u32(bars), empty = full + 8 * kStagesB, acc_full = empty + 8 * kStagesB, acc_empty = acc_full + 16;
+    const unsigned a_full = acc_empty + 16, a_empty = a_full + 8 * kSlots;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kStages; ++s) {
-            mbar_init(codes_full + 8 * s, 1);
-            mbar_init(scales_full + 8 * s, 4);
+        for (int s = 0; s < kStagesB; ++s) {
+            mbar_init(full + 8 * s, 1);
             mbar_init(empty + 8 * s, 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(acc_full + 8 * b, 1);
-            mbar_init(acc_empty + 8 * b, 4);
+            mbar_init(acc_empty + 8 * b, 16);
+        }
+        for (int s = 0; s < kSlots; ++s) {
+            mbar_init(a_full + 8 * s, 1);
+            mbar_init(a_empty + 8 * s, 1);
         }
         gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         tma_prefetch_map(&tp.map_a);
         tma_prefetch_map(&tp.map_b);
+        tma_prefetch_map(&tp.map_sa);
+        tma_prefetch_map(&tp.map_sb);
+        if (tp.vec_ok) tma_prefetch_map(&tp.map_out);
     }
     if (warp == 1) tmem_alloc(smem_u32(&tmem_base), kTmemColumns);
     tc_fence_before();
     __syncthreads();
+    cluster_sync();
     tc_fence_after();
-    const unsigned tmem = tmem_base;
+    const unsigned tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
     volatile int* stop = &gave_up;
+    wait_for_previous();
 
+    // Warps 0 and 1 walk their loops whole, so that addresses and descriptors are uniform; one lane issues.  (With a
+    // loop of one lane, moving the operands to where these instructions take them bounded the product: 58 cycles for
+    // each move of scales.)
     if (warp == 0) {
-        if (lane == 0) {
-            unsigned it = 0;
-            const unsigned bytes = kStageA + tile_n * 128;
-            bool ok = true;
-            for (long long tile = blockIdx.x; ok && tile < tp.tiles; tile += gridDim.x) {
-                const int m0 = static_cast<int>(tile / tp.n_tiles) * kTileM, n0 = static_cast<int>(tile % tp.n_tiles) * tile_n;
-                for (int kt = 0; kt < tp.k_stages; ++kt, ++it) {
-                    const unsigned s = it % kStages, round = it / kStages;
-                    if (!mbar_wait(empty + 8 * s, (round & 1) ^ 1, stop)) {
-                        ok = false;
-                        break;
-                    }
-                    const unsigned a = smem + s * kStageBytes, b = a + kStageA;
-                    mbar_arrive_tx(codes_full + 8 * s, bytes);
-                    tma_load_2d(a, &tp.map_a, kt * 128, m0, codes_full + 8 * s);
-                    tma_load_2d(b, &tp.map_b, kt * 128, n0, codes_full + 8 * s);
-                }
+        const bool issue = elect_one();
+        Ring r;
+        unsigned rows = 0, started = 0;
+        const unsigned b_bytes = tile_n / 2 * 128 + kWords<FMT> * tp.groups_n * 512, a_bytes = kCodesA + kWords<FMT> * 512;
+        const unsigned full_at = at_leader(full), a_full_at = at_leader(a_full);
+        int last_m = -1;
+        bool ok = true;
+        for (Walk w(tp); ok && w.tile < w.end; w.tile += w.step) {
+            int m, n;
+            w.place(tp, m, n);
+            const int m_block = 2 * m + static_cast<int>(rank);
+            const bool new_row = tp.resident && m != last_m;
+            if (new_row) {
+                last_m = m;
+                ++rows;
             }
-            if (!ok) {  // every copy that was started lands before the CTA ends
-                int none = 0;
-                for (unsigned j = it > kStages ? it - kStages : 0; j < it; ++j) mbar_wait(codes_full + 8 * (j % kStages), (j / kStages) & 1, &none);
+            for (int kt = 0; kt < tp.k_stages; ++kt) {
+                const int sa_row = (m_block * tp.k_stages + kt) * kWords<FMT>;
+                if (new_row) {
+                    ok = mbar_wait(a_empty + 8 * kt, rows & 1, stop);
+                    if (!ok) break;
+                    if (issue) {
+                        const unsigned a = a_base + kt * a_step, bar = a_full_at + 8 * kt;
+                        if (rank == 0) mbar_arrive_tx(a_full + 8 * kt, 2 * a_bytes);
+                        tma_load_2d(a, &tp.map_a, kt * 128, m_block * kTileM, bar);
+                        tma_load_2d(a + kCodesA, &tp.map_sa, 0, sa_row, bar);
+                    }
+                    __syncwarp();
+                }
+                ok = mbar_wait(empty + 8 * r.s, r.parity ^ 1, stop);
+                if (!ok) break;
+                if (issue) {
+                    const unsigned b = b_base + r.s * b_step, bar = full_at + 8 * r.s;
+                    if (rank == 0) mbar_arrive_tx(full + 8 * r.s, 2 * (b_bytes + (tp.resident ? 0u : a_bytes)));
+                    tma_load_2d(b, &tp.map_b, kt * 128, n * tile_n + static_cast<int>(rank) * (tile_n / 2), bar);
+                    tma_load_2d(b + kCodesB, &tp.map_sb, 0, (n * tp.k_stages + kt) * kWords<FMT> * tp.groups_n, bar);
+                    if (!tp.resident) {
+                        const unsigned a = a_base + r.s * a_step;
+                        tma_load_2d(a, &tp.map_a, kt * 128, m_block * kTileM, bar);
+                        tma_load_2d(a + kCodesA, &tp.map_sa, 0, sa_row, bar);
+                    }
+                }
+                __syncwarp();
+                r.next(ring);
+                ++started;
             }
         }
-    } else if (warp == 1) {
-        if (lane == 0) {
-            // bits 4-5 / 29-30 which scales of a word, 7-9 / 10-12 type of A / B, 17-22 N / 8, 23 scale type, 24-28 M / 16
-            const unsigned type = FMT == kMxfp8 ? 0u : 1u;
-            const unsigned idesc = type << 7 | type << 10 | static_cast<unsigned>(tile_n / 8) << 17 | (FMT == kNvfp4 ? 0u : 1u << 23) | (kTileM / 16) << 24;
-            unsigned it = 0, count = 0;
-            bool ok = true;
-            for (long long tile = blockIdx.x; ok && tile < tp.tiles; tile += gridDim.x, ++count) {
-                const unsigned buf = count & 1;
-                if (!mbar_wait(acc_empty + 8 * buf, ((count >> 1) & 1) ^ 1, stop)) break;
+        if (*stop && rank == 0) {  // every copy that was started lands before the pair ends
+            int none = 0;
+            Ring back = r;
+            for (unsigned j = 0; j < ring && j < started; ++j) {
+                if (back.s == 0) back.parity ^= 1u;
+                back.s = back.s == 0 ? ring - 1 : back.s - 1;
+                mbar_wait(full + 8 * back.s, back.parity, &none);
+            }
+            for (int kt = 0; rows && kt < tp.k_stages; ++kt) mbar_wait(a_full + 8 * kt, (rows - 1) & 1, &none);
+        }
+    } else if (warp == 1 && rank == 0) {
+        const bool issue = elect_one();
+        // bits 4-5 / 29-30 which scales of a word, 7-9 / 10-12 type of A / B, 17-22 N / 8, 23 scale type, 24-28 M / 16
+        const unsigned type = FMT == kMxfp8 ? 0u : 1u;
+        const unsigned idesc = type << 7 | type << 10 | static_cast<unsigned>(tile_n / 8) << 17 | (FMT == kNvfp4 ? 0u : 1u << 23) | (2 * kTileM / 16) << 24;
+        Ring r;
+        unsigned count = 0, rows = 0;
+        int last_m = -1;
+        bool ok = true;
+        for (Walk w(tp); ok && w.tile < w.end; w.tile += w.step, ++count) {
+            int m, n;
+            w.place(tp, m, n);
+            const bool new_row = tp.resident && m != last_m;
+            // the last tile that needs this row's A frees its slots
+            const bool row_ends = tp.resident && n == tp.n_tiles - 1;
+            if (new_row) {
+                last_m = m;
+                ++rows;
+            }
+            const unsigned buf = count & 1;
+            if (!mbar_wait(acc_empty + 8 * buf, ((count >> 1) & 1) ^ 1, stop)) break;
+            tc_fence_after();
+            const unsigned d = tmem + buf * kMaxTileN;
+            for (int kt = 0; kt < tp.k_stages; ++kt) {
+                ok = (!new_row || mbar_wait(a_full + 8 * kt, (rows - 1) & 1, stop)) && mbar_wait(full + 8 * r.s, r.parity, stop);
+                if (!ok) break;
                 tc_fence_after();
-                const unsigned d = tmem + buf * kMaxTileN;
-                for (int kt = 0; kt < tp.k_stages; ++kt, ++it) {
-                    const unsigned s = it % kStages, parity = (it / kStages) & 1;
-                    if (!mbar_wait(codes_full + 8 * s, parity, stop) || !mbar_wait(scales_full + 8 * s, parity, stop)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const unsigned a = smem + s * kStageBytes, b = a + kStageA, sa = b + kStageB, sb = sa + kScaleA;
+                const unsigned a = a_base + (tp.resident ? kt : r.s) * a_step, b = b_base + r.s * b_step;
+                const unsigned sa = a + kCodesA, sb = b + kCodesB;
+                const unsigned long long da = smem_desc(a, 16, 1024, 2), db = smem_desc(b, 16, 1024, 2);
+                if (issue) {
 #pragma unroll
                     for (int g = 0; g < kWords<FMT>; ++g) {
                         copy_scales(tmem + kTmemScaleA + 4 * g, sa + 512 * g);
-                        copy_scales(tmem + kTmemScaleB + 8 * g, sb + 1024 * g);
-                        if (tile_n > 128) copy_scales(tmem + kTmemScaleB + 8 * g + 4, sb + 1024 * g + 512);
+                        copy_scales(tmem + kTmemScaleB + 8 * g, sb + 512 * g * tp.groups_n);
+                        if (tp.groups_n > 1) copy_scales(tmem + kTmemScaleB + 8 * g + 4, sb + 1024 * g + 512);
                     }
-                    const unsigned long long da = smem_desc(a, 16, 1024, 2), db = smem_desc(b, 16, 1024, 2);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int g = i * kWords<FMT> / 4;                                          // group of 4 scales
@@ -191,111 +301,92 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                         mma<FMT>(d, da + 2 * i, db + 2 * i, idesc | id << 4 | id << 29, tmem + kTmemScaleA + 4 * g, tmem + kTmemScaleB + 8 * g,
                                  kt > 0 || i > 0);
                     }
-                    tc_commit(empty + 8 * s);
+                    tc_commit(empty + 8 * r.s);
+                    if (row_ends) tc_commit(a_empty + 8 * kt);
+                    if (kt == tp.k_stages - 1) tc_commit(acc_full + 8 * buf);
                 }
-                if (ok) tc_commit(acc_full + 8 * buf);
-            }
-        }
-    } else if (warp >= 8) {
-        const int t = threadIdx.x - 256;
-        constexpr int depth = 3;  // stages of scale words on their way
-        unsigned wa[depth][4], wb0[depth][4], wb1[depth][4];
-        long long ld_tile = blockIdx.x;
-        int ld_kt = 0;
-        auto load = [&](int d) {
-            if (ld_tile >= tp.tiles) return;
-            const long long m0 = ld_tile / tp.n_tiles * kTileM;
-            const int n0 = static_cast<int>(ld_tile % tp.n_tiles) * tile_n;
-            load_scales<FMT>(p.a, m0 + t, ld_kt, wa[d]);
-            if (t < tile_n) load_scales<FMT>(p.b, n0 + t, ld_kt, wb0[d]);
-            if (t + 128 < tile_n) load_scales<FMT>(p.b, n0 + t + 128, ld_kt, wb1[d]);
-            if (++ld_kt == tp.k_stages) {
-                ld_kt = 0;
-                ld_tile += gridDim.x;
-            }
-        };
-        const long long mine = blockIdx.x < tp.tiles ? (tp.tiles - 1 - blockIdx.x) / gridDim.x + 1 : 0;
-        const long long total = mine * tp.k_stages;
-#pragma unroll
-        for (int d = 0; d < depth; ++d) load(d);
-        bool ok = true;
-        for (long long it0 = 0; ok && it0 < total; it0 += depth) {
-#pragma unroll
-            for (int d = 0; d < depth; ++d) {
-                const long long it = it0 + d;
-                if (!ok || it >= total) break;
-                const unsigned s = static_cast<unsigned>(it % kStages), round = static_cast<unsigned>(it / kStages);
-                ok = mbar_wait(empty + 8 * s, (round & 1) ^ 1, stop);
-                if (!ok) break;
-                const unsigned sa = smem + s * kStageBytes + kStageA + kStageB, sb = sa + kScaleA;
-                store_scales<FMT>(sa, 512, t, wa[d]);
-                if (t < tile_n) store_scales<FMT>(sb, 1024, t, wb0[d]);
-                if (t + 128 < tile_n) store_scales<FMT>(sb, 1024, t + 128, wb1[d]);
-                fence_async_shared();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(scales_full + 8 * s);
-                load(d);
+                r.next(ring);
             }
         }
     } else if (warp >= 4) {
-        const int quarter = warp - 4;
-        unsigned char* staging = raw + (smem - smem_u32(raw)) + kStages * kStageBytes + quarter * kStaging;
+        // Warps 4-7 and 8-11 take alternate chunks of 128 bytes of the tile's rows; warp w reads TMEM lanes 32 (w % 4)...
+        const int quarter = warp % 4, half = (warp - 4) / 4;
+        unsigned char* staging = raw + (smem - smem_u32(raw)) + kRing + (warp - 4) * kStaging;
         const float alpha = __fmul_rn(mx_tensor_scale(p.a), mx_tensor_scale(p.b));
-        constexpr int chunk = 128 / sizeof(T);  // columns staged at a time
-        const int n = static_cast<int>(p.b.rows);
+        constexpr int chunk = 128 / sizeof(T), per = 16 / sizeof(T);  // columns of a chunk, of 16 bytes
+        const int n_all = static_cast<int>(p.b.rows);
+        const unsigned acc_empty_at = at_leader(acc_empty);
         unsigned count = 0;
-        for (long long tile = blockIdx.x; tile < tp.tiles; tile += gridDim.x, ++count) {
+        for (Walk w(tp); w.tile < w.end; w.tile += w.step, ++count) {
+            int m, n;
+            w.place(tp, m, n);
             const unsigned buf = count & 1;
             if (!mbar_wait(acc_full + 8 * buf, (count >> 1) & 1, stop)) break;
             tc_fence_after();
-            const long long m0 = tile / tp.n_tiles * kTileM + quarter * 32;
-            const int n0 = static_cast<int>(tile % tp.n_tiles) * tile_n;
-            const int width = min(tile_n, n - n0);
+            const long long m0 = static_cast<long long>(2 * m + rank) * kTileM + quarter * 32;
+            const int n0 = n * tile_n, width = min(tile_n, n_all - n0);
             const int rows = static_cast<int>(min(static_cast<long long>(32), p.a.rows - m0));
             const unsigned from = tmem + (static_cast<unsigned>(quarter * 32) << 16) + buf * kMaxTileN;
-            for (int c0 = 0; c0 < tile_n; c0 += chunk) {
+            auto release = [&]() {  // this warp has read its columns of the accumulator
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_at(acc_empty_at + 8 * buf);
+            };
+            if (half * chunk >= tile_n) release();
+            for (int c0 = half * chunk; c0 < tile_n; c0 += 2 * chunk) {
+                const int groups = min(chunk, tile_n - c0) / 16;  // of 16 columns
+                const bool whole = tp.vec_ok && groups == chunk / 16;
+                unsigned v[chunk];
 #pragma unroll
-                for (int g = 0; g < chunk / 16; ++g) {
-                    if (c0 + g * 16 >= tile_n) break;
-                    unsigned v[16];
-                    tmem_load16(from + c0 + g * 16, v);
-                    tmem_load_wait();
-                    T o[16];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[i] = from_float<T>(__fmul_rn(__uint_as_float(v[i]), alpha));
-                    uint4* to = reinterpret_cast<uint4*>(staging + lane * kStagingPitch) + g * sizeof(T);
-#pragma unroll
-                    for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) to[i] = reinterpret_cast<const uint4*>(o)[i];
-                }
-                if (c0 + chunk >= tile_n) {  // the accumulator is free once its last columns are in registers
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(acc_empty + 8 * buf);
-                } else {
+                for (int g = 0; g < chunk / 16; ++g)
+                    if (g < groups) tmem_load16(from + c0 + g * 16, v + 16 * g);
+                tmem_load_wait();
+                if (c0 + 2 * chunk >= tile_n) release();  // before waiting for the stores, so that the next sums may start
+                if (whole) {
+                    if (lane == 0) tma_store_wait_read();
                     __syncwarp();
                 }
-                const int cols = min(chunk, width - c0);
-                T* out = static_cast<T*>(p.out) + m0 * n + n0 + c0;
-                if (tp.vec_ok) {
-                    const int piece = lane % 8;
-                    for (int r = lane / 8; r < rows; r += 4)
-                        if (piece * static_cast<int>(16 / sizeof(T)) < cols)
-                            reinterpret_cast<uint4*>(out + static_cast<long long>(r) * n)[piece] =
-                                reinterpret_cast<const uint4*>(staging + r * kStagingPitch)[piece];
+                T o[chunk];
+#pragma unroll
+                for (int i = 0; i < chunk; ++i) o[i] = from_float<T>(__fmul_rn(__uint_as_float(v[i]), alpha));
+                if (whole) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)  // 16-byte pieces in the order of the 128-byte swizzle
+                        reinterpret_cast<uint4*>(staging + lane * 128)[i ^ (lane & 7)] = reinterpret_cast<const uint4*>(o)[i];
+                    fence_async_shared();
+                    __syncwarp();
+                    if (lane == 0 && rows > 0 && c0 < width)
+                        tma_store_2d(&tp.map_out, (n0 + c0) * static_cast<int>(sizeof(T)), static_cast<int>(m0), smem_u32(staging));
+                } else if (tp.vec_ok) {  // the tile's last, narrower chunk
+                    T* out = static_cast<T*>(p.out) + (m0 + lane) * n_all + n0 + c0;
+                    if (lane < rows) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (i * per < groups * 16 && c0 + i * per < width) reinterpret_cast<uint4*>(out)[i] = reinterpret_cast<const uint4*>(o)[i];
+                    }
                 } else {
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) reinterpret_cast<uint4*>(staging + lane * 128)[i ^ (lane & 7)] = reinterpret_cast<const uint4*>(o)[i];
+                    __syncwarp();
+                    const int cols = min(groups * 16, width - c0);
+                    T* out = static_cast<T*>(p.out) + m0 * n_all + n0 + c0;
                     for (int r = 0; r < rows; ++r)
                         for (int c = lane; c < cols; c += 32)
-                            out[static_cast<long long>(r) * n + c] = reinterpret_cast<const T*>(staging + r * kStagingPitch)[c];
+                            out[static_cast<long long>(r) * n_all + c] = reinterpret_cast<const T*>(staging + r * 128)[((c / per) ^ (r & 7)) * per + c % per];
                 }
-                __syncwarp();
             }
         }
+        if (lane == 0) tma_store_wait_read();
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
+    cluster_sync();  // neither CTA's memory or barriers are used by the other any more
     tc_fence_after();
     if (warp == 1) tmem_free(tmem, kTmemColumns);
+    if (threadIdx.x == 0 && gave_up) atomicAdd(&g_gave_up, 1u);
 }
 
 int last_error() { return static_cast<int>(cudaGetLastError()); }
@@ -311,8 +402,18 @@ int launch_tiles(const TileParams& tp, cudaStream_t st) {
         if (e != cudaSuccess) return static_cast<int>(e);
         prepared.fetch_or(bit, std::memory_order_release);
     }
-    const long long grid = tp.tiles < kSms ? tp.tiles : kSms;
-    product_kernel<T, FMT><<<static_cast<unsigned>(grid), kThreads, kSmem, st>>>(tp);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(2 * (tp.tiles < kSms / 2 ? tp.tiles : kSms / 2)));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // set up while arrange_kernel runs
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, product_kernel<T, FMT>, tp);
+    if (e != cudaSuccess) return static_cast<int>(e);
     mx_count_launch();
     return last_error();
 }
@@ -324,11 +425,38 @@ int by_format(const TileParams& tp, cudaStream_t st) {
     return launch_tiles<T, kMxfp8>(tp, st);
 }
 
+int words_of(int fmt) { return fmt == kNvfp4 ? 4 : fmt == kMxfp4 ? 2 : 1; }
+
+// Sizes of a product's tiles, a function of its shape and format alone.
+void plan(TileParams& tp) {
+    const MxProduct& p = tp.p;
+    tp.m_tiles = (p.a.rows + 2 * kTileM - 1) / (2 * kTileM);
+    const int n = static_cast<int>(p.b.rows);
+    // The width that needs the least time: rounds of tiles over the pairs, each costing its width and a fixed part.
+    // Where the result's bytes weigh most (few stages a tile), tiles of whole 128-byte lines: two tiles that share lines
+    // write them at different times (50176 x 4096 x 1024: 197 us with 208 columns, 183 with 192; 8192^3, where 224
+    // columns copy less for each product: 224 us against 250 with 192).
+    long long best = 0;
+    const int line = p.out_dtype == kF32 ? 32 : 64;
+    tp.k_stages = (mx_code_pitch(p.a.format, p.a.cols) + 127) / 128;
+    tp.resident = tp.k_stages <= kSlots;
+    for (int w = 16; w <= kMaxTileN; w += 16) {
+        if (tp.resident && w % line && w < n && w > line) continue;
+        const long long tiles = tp.m_tiles * ((n + w - 1) / w), cost = (tiles + kSms / 2 - 1) / (kSms / 2) * (w + 32);
+        if (best == 0 || cost <= best) best = cost, tp.tile_n = w;
+    }
+    tp.n_tiles = (n + tp.tile_n - 1) / tp.tile_n;
+    tp.groups_n = tp.tile_n > 128 ? 2 : 1;
+    tp.tiles = tp.m_tiles * tp.n_tiles;
+}
+long long groups_a(const TileParams& tp) { return 2 * tp.m_tiles * tp.k_stages * words_of(tp.p.a.format); }
+long long groups_b(const TileParams& tp) { return static_cast<long long>(tp.n_tiles) * tp.groups_n * tp.k_stages * words_of(tp.p.a.format); }
+
 }  // namespace
 
 // cuTensorMapEncodeTiled, reached through the runtime so that the library does not link libcuda.
-int mx_encode_map(void* map, int dtype_16, const void* base, unsigned long long inner, unsigned long long rows, unsigned long long pitch,
-                  unsigned box_inner, unsigned box_rows) {
+int mx_encode_map(void* map, int element_bytes, const void* base, unsigned long long inner, unsigned long long rows, unsigned long long pitch,
+                  unsigned box_inner, unsigned box_rows, int swizzle) {
     using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
     static std::atomic<Encode> encode{nullptr};
@@ -344,34 +472,50 @@ int mx_encode_map(void* map, int dtype_16, const void* base, unsigned long long 
     }
     const cuuint64_t dims[2] = {inner, rows}, strides[1] = {pitch};
     const cuuint32_t box[2] = {box_inner, box_rows}, step[2] = {1, 1};
-    const CUresult r = f(static_cast<CUtensorMap*>(map), dtype_16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2,
-                         const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUtensorMapDataType type = element_bytes == 1   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                     : element_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                          : CU_TENSOR_MAP_DATA_TYPE_UINT32;
+    const CUresult r = f(static_cast<CUtensorMap*>(map), type, 2, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? 0 : static_cast<int>(cudaErrorInvalidValue);
 }
 
-size_t mx_matmul_workspace(const MxProduct&) { return 0; }
+int mx_gave_up(unsigned* count) { return static_cast<int>(cudaMemcpyFromSymbol(count, g_gave_up, sizeof *count)); }
+
+size_t mx_matmul_workspace(const MxProduct& p) {
+    if (p.a.rows == 0 || p.b.rows == 0) return 0;
+    TileParams tp{};
+    tp.p = p;
+    plan(tp);
+    return static_cast<size_t>(groups_a(tp) + groups_b(tp)) * 512;
+}
 
 int launch_mx_matmul(const MxProduct& p, void* stream) {
     TileParams tp{};
     tp.p = p;
-    const int fmt = p.a.format, pitch = mx_code_pitch(fmt, p.a.cols);
-    const long long m_tiles = (p.a.rows + kTileM - 1) / kTileM;
-    const int n = static_cast<int>(p.b.rows);
-    // The width that needs the least time: rounds of tiles over the SMs, each costing its width and a fixed part.
-    long long best = 0;
-    for (int w = 16; w <= kMaxTileN; w += 16) {
-        const long long tiles = m_tiles * ((n + w - 1) / w), cost = (tiles + kSms - 1) / kSms * (w + 32);
-        if (best == 0 || cost <= best) best = cost, tp.tile_n = w;
-    }
-    tp.n_tiles = (n + tp.tile_n - 1) / tp.tile_n;
-    tp.tiles = m_tiles * tp.n_tiles;
-    tp.k_stages = (pitch + 127) / 128;
-    const int esz = p.out_dtype == kF32 ? 4 : 2;
-    tp.vec_ok = static_cast<long long>(n) * esz % 16 == 0;
-    if (int e = mx_encode_map(&tp.map_a, 0, p.a.codes, pitch, p.a.rows, pitch, 128, kTileM)) return e;
-    if (int e = mx_encode_map(&tp.map_b, 0, p.b.codes, pitch, n, pitch, 128, tp.tile_n)) return e;
+    plan(tp);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int fmt = p.a.format, pitch = mx_code_pitch(fmt, p.a.cols), words = words_of(fmt), n = static_cast<int>(p.b.rows);
+    const int esz = p.out_dtype == kF32 ? 4 : 2;
+    const long long out_pitch = static_cast<long long>(n) * esz, ga = groups_a(tp), gb = groups_b(tp);
+    if (ga > 0x7fffffffll || gb > 0x7fffffffll) return static_cast<int>(cudaErrorInvalidValue);
+    tp.vec_ok = out_pitch % 16 == 0;
+    unsigned char* sa = static_cast<unsigned char*>(p.workspace);
+    unsigned char* sb = sa + ga * 512;
+    if (int e = mx_encode_map(&tp.map_a, 1, p.a.codes, pitch, p.a.rows, pitch, 128, kTileM, 1)) return e;
+    if (int e = mx_encode_map(&tp.map_b, 1, p.b.codes, pitch, n, pitch, 128, tp.tile_n / 2, 1)) return e;
+    if (int e = mx_encode_map(&tp.map_sa, 4, sa, 128, ga, 512, 128, words, 0)) return e;
+    if (int e = mx_encode_map(&tp.map_sb, 4, sb, 128, gb, 512, 128, words * tp.groups_n, 0)) return e;
+    if (tp.vec_ok)
+        if (int e = mx_encode_map(&tp.map_out, 1, p.out, out_pitch, p.a.rows, out_pitch, 128, 32, 1)) return e;
+    Arrange a{p.a, reinterpret_cast<unsigned*>(sa), kTileM, 1, tp.k_stages * words, 0}, b{p.b, reinterpret_cast<unsigned*>(sb), tp.tile_n, tp.groups_n, tp.k_stages * words, 0};
+    const int quads = (a.words + 3) / 4;
+    a.threads = 2 * tp.m_tiles * 32 * quads;
+    b.threads = static_cast<long long>(tp.n_tiles) * tp.groups_n * 32 * quads;
+    arrange_kernel<<<static_cast<unsigned>((a.threads + b.threads + 255) / 256), 256, 0, st>>>(a, b);
+    mx_count_launch();
+    if (int e = last_error()) return e;
     if (p.out_dtype == kF32) return by_format<float>(tp, st);
     if (p.out_dtype == kBf16) return by_format<__nv_bfloat16>(tp, st);
     return by_format<__half>(tp, st);

@@ -56,6 +56,7 @@ struct MxProduct {
     int out_dtype;
     void* workspace;
 };
+int mx_gave_up(unsigned* count);  // products and gradients on this device that gave up a bounded wait
 size_t mx_matmul_workspace(const MxProduct& p);
 int launch_mx_matmul(const MxProduct& p, void* stream);
 

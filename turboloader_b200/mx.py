@@ -19,7 +19,7 @@ import torch
 
 from . import _capi
 
-__all__ = ["MxTensor", "MxCache", "mx_quantize", "mx_dequantize", "mx_matmul", "mx_linear"]
+__all__ = ["MxTensor", "MxCache", "mx_quantize", "mx_dequantize", "mx_matmul", "mx_linear", "mx_incomplete"]
 
 _FORMATS = {"nvfp4": 0, "mxfp4": 1, "mxfp8": 2}
 _BLOCK = (16, 32, 32)
@@ -256,6 +256,14 @@ def mx_matmul(a, b, dtype=torch.bfloat16, *, out=None, stream=None):
         _capi.check(lib.tlb_mx_matmul(C.byref(sa), C.byref(sb), out.data_ptr(), dt, ws.data_ptr() if ws is not None else None,
                                       size, handle))
     return out
+
+
+def mx_incomplete() -> int:
+    """Products and gradients on the current device whose kernels gave up a bounded wait and left their result
+    incomplete, since the library was loaded (synchronises): 0 in a healthy process."""
+    count = C.c_uint32(0)
+    _capi.check(_capi.load().tlb_mx_incomplete(C.byref(count)))
+    return int(count.value)
 
 
 def _grad(g, q, transpose, dtype):
