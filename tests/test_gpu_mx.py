@@ -5,7 +5,6 @@ import torch
 
 import turboloader_b200 as tb
 from mx_reference import BLOCK, decode, encode
-from turboloader_b200 import _capi
 
 pytestmark = pytest.mark.gpu
 
@@ -502,4 +501,4 @@ def test_launches_are_counted():
     q = tb.mx_quantize(torch.randn(4, 64, device="cuda"))
     q.dequantize()
     assert tb.launch_count() == before + 2
-    assert _capi.load().tlb_mx_matmul_workspace is not None
+    assert tb.mx_incomplete() == 0

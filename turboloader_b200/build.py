@@ -13,9 +13,9 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.environ.get("TLB_LIB") or os.path.join(HERE, "libturboloader_b200.so")
-SOURCES = ["fused_transform.cu", "host_gather.cu", "video_yuv420.cu", "antialias.cu", "normalize_copy.cu", "mx_rows.cu", "mx_matmul.cu", "mx_grad.cu",
+SOURCES = ["fused_transform.cu", "host_gather.cu", "video_yuv420.cu", "antialias.cu", "normalize_copy.cu", "mx_rows.cu", "mx_matmul.cu", "mx_few.cu", "mx_grad.cu",
            "mx_capi.cu", "capi.cu", "sharding.cpp"]
-HEADERS = ["fused_params.h", "host_gather.h", "video_params.h", "antialias_params.h", "mx_params.h", "mx_device.cuh", "mx_tma.cuh",
+HEADERS = ["fused_params.h", "host_gather.h", "video_params.h", "antialias_params.h", "mx_params.h", "mx_device.cuh", "mx_tma.cuh", "mx_tile.cuh",
            os.path.join("..", "..", "include", "turboloader_b200.h")]
 
 NVCC_FLAGS = [

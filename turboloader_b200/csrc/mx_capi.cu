@@ -118,6 +118,7 @@ int check_grad(int g_dtype, int64_t m, int32_t n, const tlb_mx_rows* q, int32_t 
     if (int rc = check_dtype(out_dtype, "out")) return rc;
     if (m < 0 || n < 0) return fail(TLB_ERR_INVALID_ARG, "g is %lld x %d", static_cast<long long>(m), n);
     if (m > TLB_MX_MAX_ROWS || n > TLB_MX_MAX_COLS) return fail(TLB_ERR_TOO_LARGE, "g: %lld x %d is too large", static_cast<long long>(m), n);
+    if (m > 0x7fffff00ll / 3) return fail(TLB_ERR_TOO_LARGE, "g: %lld rows are too many", static_cast<long long>(m));
     if (transpose != 0 && transpose != 1) return fail(TLB_ERR_INVALID_ARG, "transpose = %d must be 0 or 1", transpose);
     if (q->rows != (transpose ? m : n)) return fail(TLB_ERR_INVALID_ARG, "q has %lld rows, the sum runs over %lld", static_cast<long long>(q->rows), static_cast<long long>(transpose ? m : n));
     return TLB_OK;

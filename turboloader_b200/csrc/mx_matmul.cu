@@ -20,7 +20,7 @@
 #include <atomic>
 
 #include "mx_device.cuh"
-#include "mx_tma.cuh"
+#include "mx_tile.cuh"
 
 namespace tlb {
 namespace {
@@ -32,7 +32,6 @@ constexpr int kStages = 5, kStageBytes = kCodesA + kScaleA + kCodesB + kScaleB;
 constexpr int kSlots = 4, kSlotBytes = kCodesA + kScaleA, kStagesB = 6, kStageBBytes = kCodesB + kScaleB;
 constexpr int kRing = kSlots * kSlotBytes + kStagesB * kStageBBytes;
 static_assert(kStages * kStageBytes <= kRing && kStageBytes % 1024 == 0 && kSlotBytes % 1024 == 0 && kStageBBytes % 1024 == 0, "layout");
-constexpr int kStaging = 32 * 128;  // an epilogue warp's 32 rows of 128 bytes
 constexpr int kSmem = 1024 + kRing + 8 * kStaging;
 constexpr int kThreads = 384;
 static_assert(kSmem <= 227 * 1024 - 512, "shared memory");
@@ -60,14 +59,6 @@ struct Walk {
     __device__ void place(const TileParams& tp, int& m, int& n) const {
         m = static_cast<int>(tile / tp.n_tiles);
         n = static_cast<int>(tile - static_cast<long long>(m) * tp.n_tiles);
-    }
-};
-
-// A ring position and its parity.
-struct Ring {
-    unsigned s = 0, parity = 0;
-    __device__ void next(unsigned stages) {
-        if (++s == stages) s = 0, parity ^= 1u;
     }
 };
 
@@ -249,11 +240,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
         }
         if (*stop && rank == 0) {  // every copy that was started lands before the pair ends
             int none = 0;
-            Ring back = r;
             for (unsigned j = 0; j < ring && j < started; ++j) {
-                if (back.s == 0) back.parity ^= 1u;
-                back.s = back.s == 0 ? ring - 1 : back.s - 1;
-                mbar_wait(full + 8 * back.s, back.parity, &none);
+                r.back(ring);
+                mbar_wait(full + 8 * r.s, r.parity, &none);
             }
             for (int kt = 0; rows && kt < tp.k_stages; ++kt) mbar_wait(a_full + 8 * kt, (rows - 1) & 1, &none);
         }
@@ -310,11 +299,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
             }
         }
     } else if (warp >= 4) {
-        // Warps 4-7 and 8-11 take alternate chunks of 128 bytes of the tile's rows; warp w reads TMEM lanes 32 (w % 4)...
         const int quarter = warp % 4, half = (warp - 4) / 4;
-        unsigned char* staging = raw + (smem - smem_u32(raw)) + kRing + (warp - 4) * kStaging;
+        const unsigned staging = smem + kRing + (warp - 4) * kStaging;
         const float alpha = __fmul_rn(mx_tensor_scale(p.a), mx_tensor_scale(p.b));
-        constexpr int chunk = 128 / sizeof(T), per = 16 / sizeof(T);  // columns of a chunk, of 16 bytes
         const int n_all = static_cast<int>(p.b.rows);
         const unsigned acc_empty_at = at_leader(acc_empty);
         unsigned count = 0;
@@ -325,58 +312,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
             if (!mbar_wait(acc_full + 8 * buf, (count >> 1) & 1, stop)) break;
             tc_fence_after();
             const long long m0 = static_cast<long long>(2 * m + rank) * kTileM + quarter * 32;
-            const int n0 = n * tile_n, width = min(tile_n, n_all - n0);
-            const int rows = static_cast<int>(min(static_cast<long long>(32), p.a.rows - m0));
-            const unsigned from = tmem + (static_cast<unsigned>(quarter * 32) << 16) + buf * kMaxTileN;
-            auto release = [&]() {  // this warp has read its columns of the accumulator
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive_at(acc_empty_at + 8 * buf);
-            };
-            if (half * chunk >= tile_n) release();
-            for (int c0 = half * chunk; c0 < tile_n; c0 += 2 * chunk) {
-                const int groups = min(chunk, tile_n - c0) / 16;  // of 16 columns
-                const bool whole = tp.vec_ok && groups == chunk / 16;
-                unsigned v[chunk];
-#pragma unroll
-                for (int g = 0; g < chunk / 16; ++g)
-                    if (g < groups) tmem_load16(from + c0 + g * 16, v + 16 * g);
-                tmem_load_wait();
-                if (c0 + 2 * chunk >= tile_n) release();  // before waiting for the stores, so that the next sums may start
-                if (whole) {
-                    if (lane == 0) tma_store_wait_read();
-                    __syncwarp();
-                }
-                T o[chunk];
-#pragma unroll
-                for (int i = 0; i < chunk; ++i) o[i] = from_float<T>(__fmul_rn(__uint_as_float(v[i]), alpha));
-                if (whole) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)  // 16-byte pieces in the order of the 128-byte swizzle
-                        reinterpret_cast<uint4*>(staging + lane * 128)[i ^ (lane & 7)] = reinterpret_cast<const uint4*>(o)[i];
-                    fence_async_shared();
-                    __syncwarp();
-                    if (lane == 0 && rows > 0 && c0 < width)
-                        tma_store_2d(&tp.map_out, (n0 + c0) * static_cast<int>(sizeof(T)), static_cast<int>(m0), smem_u32(staging));
-                } else if (tp.vec_ok) {  // the tile's last, narrower chunk
-                    T* out = static_cast<T*>(p.out) + (m0 + lane) * n_all + n0 + c0;
-                    if (lane < rows) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (i * per < groups * 16 && c0 + i * per < width) reinterpret_cast<uint4*>(out)[i] = reinterpret_cast<const uint4*>(o)[i];
-                    }
-                } else {
-                    __syncwarp();
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) reinterpret_cast<uint4*>(staging + lane * 128)[i ^ (lane & 7)] = reinterpret_cast<const uint4*>(o)[i];
-                    __syncwarp();
-                    const int cols = min(groups * 16, width - c0);
-                    T* out = static_cast<T*>(p.out) + m0 * n_all + n0 + c0;
-                    for (int r = 0; r < rows; ++r)
-                        for (int c = lane; c < cols; c += 32)
-                            out[static_cast<long long>(r) * n_all + c] = reinterpret_cast<const T*>(staging + r * 128)[((c / per) ^ (r & 7)) * per + c % per];
-                }
-            }
+            const int n0 = n * tile_n;
+            const TileOut<T> to{&tp.map_out, static_cast<T*>(p.out), n_all, m0, static_cast<int>(min(32ll, p.a.rows - m0)), n0, min(tile_n, n_all - n0),
+                                tp.vec_ok};
+            write_tile(to, tmem + (static_cast<unsigned>(quarter * 32) << 16) + buf * kMaxTileN, tile_n, half, lane, staging, alpha,
+                       acc_empty_at + 8 * buf);
         }
         if (lane == 0) tma_store_wait_read();
     }
@@ -481,10 +421,16 @@ int mx_encode_map(void* map, int element_bytes, const void* base, unsigned long 
     return r == CUDA_SUCCESS ? 0 : static_cast<int>(cudaErrorInvalidValue);
 }
 
-int mx_gave_up(unsigned* count) { return static_cast<int>(cudaMemcpyFromSymbol(count, g_gave_up, sizeof *count)); }
+int mx_gave_up(unsigned* count) {
+    unsigned grads = 0;
+    if (const cudaError_t e = cudaMemcpyFromSymbol(count, g_gave_up, sizeof *count); e != cudaSuccess) return static_cast<int>(e);
+    if (const int e = mx_grad_gave_up(&grads)) return e;
+    *count += grads;
+    return 0;
+}
 
 size_t mx_matmul_workspace(const MxProduct& p) {
-    if (p.a.rows == 0 || p.b.rows == 0) return 0;
+    if (p.b.rows == 0 || mx_few(p)) return 0;
     TileParams tp{};
     tp.p = p;
     plan(tp);
@@ -492,6 +438,7 @@ size_t mx_matmul_workspace(const MxProduct& p) {
 }
 
 int launch_mx_matmul(const MxProduct& p, void* stream) {
+    if (mx_few(p)) return launch_mx_few(p, stream);
     TileParams tp{};
     tp.p = p;
     plan(tp);

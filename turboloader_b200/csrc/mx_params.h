@@ -56,6 +56,8 @@ struct MxProduct {
     int out_dtype;
     void* workspace;
 };
+bool mx_few(const MxProduct& p);  // whether launch_mx_few takes the product
+int launch_mx_few(const MxProduct& p, void* stream);
 int mx_gave_up(unsigned* count);  // products and gradients on this device that gave up a bounded wait
 size_t mx_matmul_workspace(const MxProduct& p);
 int launch_mx_matmul(const MxProduct& p, void* stream);
@@ -72,6 +74,10 @@ struct MxGrad {
     int out_dtype;
     void* workspace;
 };
+// A 2-D tensor map (cuTensorMapEncodeTiled); a cudaError_t value.
+int mx_encode_map(void* map, int element_bytes, const void* base, unsigned long long inner, unsigned long long rows, unsigned long long pitch,
+                  unsigned box_inner, unsigned box_rows, int swizzle);
+int mx_grad_gave_up(unsigned* count);
 size_t mx_grad_workspace(const MxGrad& p);
 int launch_mx_grad(const MxGrad& p, void* stream);
 

@@ -1,0 +1,107 @@
+// What the tensor-core kernels of the microscaled operators share: ring positions, and the way of a finished
+// accumulator to global memory.
+#pragma once
+#include "mx_device.cuh"
+#include "mx_tma.cuh"
+
+namespace tlb {
+
+// A ring position and its parity.
+struct Ring {
+    unsigned s = 0, parity = 0;
+    __device__ void next(unsigned stages) {
+        if (++s == stages) s = 0, parity ^= 1u;
+    }
+    __device__ void back(unsigned stages) {
+        if (s == 0) s = stages, parity ^= 1u;
+        --s;
+    }
+};
+
+constexpr int kStaging = 32 * 128;  // an epilogue warp's 32 rows of 128 bytes
+
+template <typename T>
+struct TileOut {
+    const CUtensorMap* map;  // of the whole output, boxes of 32 rows of 128 bytes, 128-byte swizzle
+    T* out;
+    long long pitch;         // elements between output rows
+    long long m0;            // the warp's first output row, and how many of its 32 there are
+    int rows;
+    int n0, width;           // the tile's first output column, and how many of its columns there are
+    int vec_ok;              // rows are multiples of 16 bytes
+};
+
+// One warp's part of a tile: the 32 rows of its TMEM lanes (`from`: its lane bits and first column), every
+// second chunk of 128 bytes of them, beginning with chunk `half`.  Arrives on `released` (of the leader) once
+// its last columns are in registers, so that the next sums may start before the stores are done.
+template <typename T>
+__device__ __forceinline__ void write_tile(const TileOut<T>& to, unsigned from, int tile_n, int half, int lane, unsigned staging, float alpha,
+                                           unsigned released) {
+    constexpr int chunk = 128 / sizeof(T), per = 16 / sizeof(T);  // columns of a chunk, of 16 bytes
+    auto release = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_at(released);
+    };
+    if (half * chunk >= tile_n) release();
+    for (int c0 = half * chunk; c0 < tile_n; c0 += 2 * chunk) {
+        const int groups = min(chunk, tile_n - c0) / 16;  // of 16 columns
+        const bool whole = to.vec_ok && groups == chunk / 16;
+        unsigned v[chunk];
+#pragma unroll
+        for (int g = 0; g < chunk / 16; ++g)
+            if (g < groups) tmem_load16(from + c0 + g * 16, v + 16 * g);
+        tmem_load_wait();
+        if (c0 + 2 * chunk >= tile_n) release();
+        if (whole) {
+            if (lane == 0) tma_store_wait_read();
+            __syncwarp();
+        }
+        T o[chunk];
+#pragma unroll
+        for (int i = 0; i < chunk; ++i) o[i] = from_float<T>(__fmul_rn(__uint_as_float(v[i]), alpha));
+        const uint4* pieces = reinterpret_cast<const uint4*>(o);
+        auto stage = [&]() {  // 16-byte pieces in the order of the 128-byte swizzle
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(staging + lane * 128 + ((i ^ (lane & 7)) * 16)), "r"(pieces[i].x),
+                             "r"(pieces[i].y), "r"(pieces[i].z), "r"(pieces[i].w)
+                             : "memory");
+        };
+        if (whole) {
+            stage();
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0 && to.rows > 0 && c0 < to.width)
+                tma_store_2d(to.map, (to.n0 + c0) * static_cast<int>(sizeof(T)), static_cast<int>(to.m0), staging);
+        } else if (to.vec_ok) {  // the tile's last, narrower chunk
+            T* out = to.out + (to.m0 + lane) * to.pitch + to.n0 + c0;
+            if (lane < to.rows) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i * per < groups * 16 && c0 + i * per < to.width) reinterpret_cast<uint4*>(out)[i] = pieces[i];
+            }
+        } else {
+            __syncwarp();
+            stage();
+            __syncwarp();
+            const int cols = min(groups * 16, to.width - c0);
+            T* out = to.out + to.m0 * to.pitch + to.n0 + c0;
+            for (int r = 0; r < to.rows; ++r)
+                for (int c = lane; c < cols; c += 32) {
+                    const unsigned at = staging + r * 128 + ((c / per) ^ (r & 7)) * 16 + c % per * static_cast<int>(sizeof(T));
+                    if constexpr (sizeof(T) == 4) {
+                        unsigned bits;
+                        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(bits) : "r"(at));
+                        reinterpret_cast<unsigned*>(out)[static_cast<long long>(r) * to.pitch + c] = bits;
+                    } else {
+                        unsigned short bits;
+                        asm volatile("ld.shared.b16 %0, [%1];" : "=h"(bits) : "r"(at));
+                        reinterpret_cast<unsigned short*>(out)[static_cast<long long>(r) * to.pitch + c] = bits;
+                    }
+                }
+        }
+    }
+}
+
+}  // namespace tlb
