@@ -23,6 +23,7 @@ __all__ = ["MxTensor", "MxCache", "mx_quantize", "mx_dequantize", "mx_matmul", "
 
 _FORMATS = {"nvfp4": 0, "mxfp4": 1, "mxfp8": 2}
 _BLOCK = (16, 32, 32)
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the handle alone: a Stream object costs 3 us a call
 _DTYPES = {torch.float32: _capi.TLB_F32, torch.bfloat16: _capi.TLB_BF16, torch.float16: _capi.TLB_F16}
 
 
@@ -66,6 +67,8 @@ def _table(t, dtype, n, device, what):
 
 
 def _check_scale(scale, device):
+    if type(scale) is float and 0.0 < scale < float("inf"):
+        return scale
     if isinstance(scale, torch.Tensor):
         if scale.device != device or scale.dtype != torch.float32 or scale.numel() != 1:
             raise TypeError(f"a scale tensor must be one float32 value on {device}")
@@ -103,7 +106,7 @@ class _Here:
 def _on(device, stream):
     """Context in which the library is called for tensors of ``device``: gives the raw stream."""
     if stream is None and torch.cuda.current_device() == device.index:
-        return _Here(torch.cuda.current_stream().cuda_stream)
+        return _Here(_raw_stream(device.index))
     if stream is not None and stream.device != device:
         raise ValueError(f"stream is on {stream.device}, the tensors on {device}")
     return _elsewhere(device, stream)
@@ -149,6 +152,13 @@ class MxTensor:
         self.codes, self.scales, self.shape, self.format = codes, scales, shape, format
         self.scale = 1.0 if scale == 1.0 and not isinstance(scale, torch.Tensor) else _check_scale(scale, codes.device)
 
+    @classmethod
+    def _made(cls, codes, scales, shape, rows, format, fmt, scale):
+        """Of tensors that this module made."""
+        self = object.__new__(cls)
+        self.codes, self.scales, self.shape, self.format, self.scale, self._fmt, self._rows = codes, scales, shape, format, scale, fmt, rows
+        return self
+
     @property
     def device(self):
         return self.codes.device
@@ -164,7 +174,7 @@ class MxTensor:
 
 
 def _as_rows(x, what):
-    """(data, rows, cols, row pitch) of (..., cols) values whose rows lie at equal distances."""
+    """(rows, cols, row pitch) of (..., cols) values whose rows lie at equal distances."""
     _cuda(x, what)
     if x.dim() < 1:
         raise ValueError(f"{what} must have at least one dimension")
@@ -191,7 +201,10 @@ def mx_quantize(x, format="nvfp4", *, scale=1.0, stream=None):
     contiguous and the rows equally spaced (a slice of a wider matrix will do).  ``scale``: the tensor scale
     that values are divided by first, a float or one float32 value on the device; a power of two loses
     nothing.  For ``nvfp4``, ``max|x| / 2688`` rounded up to a power of two uses the range of its scales."""
-    fmt = _format_id(format)
+    return _quantize(x, format, _format_id(format), scale, stream)
+
+
+def _quantize(x, format, fmt, scale, stream=None):
     rows, cols, pitch = _as_rows(x, "x")
     dt = _dtype_id(x.dtype, "x")
     cp, sp = _pitches(fmt, cols)
@@ -200,8 +213,8 @@ def mx_quantize(x, format="nvfp4", *, scale=1.0, stream=None):
     with _on(device, stream) as handle:
         codes = torch.empty((rows, cp), dtype=torch.uint8, device=device)
         scales = torch.empty((rows, sp), dtype=torch.uint8, device=device)
-        q = MxTensor(codes, scales, x.shape, format, scale=scale)
-        _capi.check(_capi.load().tlb_mx_quantize(C.byref(q._struct()), x.data_ptr(), dt, pitch, handle))
+        q = MxTensor._made(codes, scales, tuple(x.shape), rows, format, fmt, scale)
+        _capi.check(_capi.load().tlb_mx_quantize(q._struct(), x.data_ptr(), dt, pitch, handle))
     return q
 
 
@@ -222,7 +235,7 @@ def mx_dequantize(q, dtype=torch.float32, *, out=None, stream=None):
     with _on(q.device, stream) as handle:
         out = _out(out, q.shape, dtype, q.device)
         cache = _capi.MxCache(q._struct(), 1, None, None, None)
-        _capi.check(_capi.load().tlb_mx_read(C.byref(cache), None, q._rows, out.data_ptr(), dt, None, handle))
+        _capi.check(_capi.load().tlb_mx_read(cache, None, q._rows, out.data_ptr(), dt, None, handle))
     return out
 
 
@@ -245,16 +258,18 @@ def mx_matmul(a, b, dtype=torch.bfloat16, *, out=None, stream=None):
     """``a`` (..., k) times the transpose of ``b`` (n, k), two ``MxTensor`` of one format: (..., n) of ``dtype``.
     The products of the codes enter whole and are summed in fp32; the result is rounded once."""
     _check_pair(a, b)
-    dt = _dtype_id(dtype, "dtype")
+    return _matmul(a, b, dtype, _dtype_id(dtype, "dtype"), out, stream)
+
+
+def _matmul(a, b, dtype, dt, out=None, stream=None):
     lib = _capi.load()
-    device = a.device
+    device = a.codes.device
     with _on(device, stream) as handle:
         out = _out(out, (*a.shape[:-1], b.shape[0]), dtype, device)
         sa, sb = a._struct(), b._struct()
-        size = lib.tlb_mx_matmul_workspace(C.byref(sa), C.byref(sb), dt)
+        size = lib.tlb_mx_matmul_workspace(sa, sb, dt)
         ws = _workspace(size, device)
-        _capi.check(lib.tlb_mx_matmul(C.byref(sa), C.byref(sb), out.data_ptr(), dt, ws.data_ptr() if ws is not None else None,
-                                      size, handle))
+        _capi.check(lib.tlb_mx_matmul(sa, sb, out.data_ptr(), dt, None if ws is None else ws.data_ptr(), size, handle))
     return out
 
 
@@ -275,10 +290,10 @@ def _grad(g, q, transpose, dtype):
     with _on(device, None) as handle:
         out = torch.empty((n if transpose else m, q.shape[-1]), dtype=dtype, device=device)
         sq = q._struct()
-        size = lib.tlb_mx_grad_workspace(gt, m, n, C.byref(sq), transpose, dt)
+        size = lib.tlb_mx_grad_workspace(gt, m, n, sq, transpose, dt)
         ws = _workspace(size, device)
-        _capi.check(lib.tlb_mx_grad(g.data_ptr(), gt, m, n, C.byref(sq), transpose, out.data_ptr(), dt,
-                                    ws.data_ptr() if ws is not None else None, size, handle))
+        _capi.check(lib.tlb_mx_grad(g.data_ptr(), gt, m, n, sq, transpose, out.data_ptr(), dt, None if ws is None else ws.data_ptr(), size,
+                                    handle))
     return out
 
 
@@ -295,30 +310,33 @@ def _spaced(x):
 class _MxLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, held_x, held_w, format, scale, weight_scale, dtype):
-        qx = held_x if x is None else mx_quantize(_spaced(x), format, scale=scale)
-        qw = held_w if weight is None else mx_quantize(_spaced(weight), format, scale=weight_scale)
-        y = mx_matmul(qx, qw, dtype)
-        ctx.x_dtype = None if x is None else x.dtype
-        ctx.w_dtype = None if weight is None else weight.dtype
-        keep_x, keep_w = weight is not None and ctx.needs_input_grad[1], x is not None and ctx.needs_input_grad[0]
-        ctx.held = [(q.shape, q.format, q.scale) if keep else None for q, keep in ((qx, keep_x), (qw, keep_w))]
-        ctx.x_shape = qx.shape
-        ctx.save_for_backward(*([qx.codes, qx.scales] if keep_x else []), *([qw.codes, qw.scales] if keep_w else []))
-        return y
+        fmt = _FORMATS[format]
+        qx = held_x if x is None else _quantize(_spaced(x), format, fmt, scale)
+        qw = held_w if weight is None else _quantize(_spaced(weight), format, fmt, weight_scale)
+        needs_x, needs_w = ctx.needs_input_grad[:2]
+        # the gradient of one operand needs the other's codes
+        saved, held = [], []
+        for q, keep in ((qx, needs_w), (qw, needs_x)):
+            held.append((q.shape, q._rows, q.scale) if keep else None)
+            if keep:
+                saved += [q.codes, q.scales]
+        ctx.save_for_backward(*saved)
+        ctx.held, ctx.format, ctx.x_shape = held, format, qx.shape
+        ctx.types = (x.dtype if needs_x else None, weight.dtype if needs_w else None)
+        return _matmul(qx, qw, dtype, _DTYPES[dtype])
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         saved = list(ctx.saved_tensors)
-        kept = []
-        for held in ctx.held:
-            kept.append(None if held is None else MxTensor(saved.pop(0), saved.pop(0), held[0], held[1], scale=held[2]))
-        qx, qw = kept
-        g = g.reshape(-1, g.shape[-1]).contiguous()
+        qx, qw = (None if h is None else MxTensor._made(saved.pop(0), saved.pop(0), h[0], h[1], ctx.format, _FORMATS[ctx.format], h[2])
+                  for h in ctx.held)
+        if g.dim() != 2 or not g.is_contiguous():
+            g = g.reshape(-1, g.shape[-1]).contiguous()
         if g.data_ptr() % 16:
             g = g.clone()
-        gx = _grad(g, qw, 0, ctx.x_dtype).view(ctx.x_shape) if qw is not None else None
-        gw = _grad(g, qx, 1, ctx.w_dtype) if qx is not None else None
+        gx = _grad(g, qw, 0, ctx.types[0]).view(ctx.x_shape) if qw is not None else None
+        gw = _grad(g, qx, 1, ctx.types[1]) if qx is not None else None
         return gx, gw, None, None, None, None, None, None
 
 
@@ -361,6 +379,7 @@ class MxCache:
 
     def __init__(self, codes, scales, cols, format, *, lengths=None, scale=1.0, status=None):
         self._fmt = _format_id(format)
+        self._owner = None
         _cuda(codes, "codes")
         if codes.dim() != 3:
             raise ValueError("codes must be (slots, tokens, code pitch)")
@@ -372,7 +391,6 @@ class MxCache:
         self.lengths = None if lengths is None else _table(lengths, torch.int32, self.slots, codes.device, "lengths")
         self.scale = _check_scale(scale, codes.device)
         self.status = None if status is None else _table(status, torch.int32, 1, codes.device, "status")
-        self._owner = None
 
     @classmethod
     def empty(cls, slots, tokens, cols, format="nvfp4", *, ragged=False, scale=1.0, device=None):
@@ -431,7 +449,7 @@ class MxCache:
                 if torch.cuda.is_current_stream_capturing():
                     raise RuntimeError(f"write more than {_capi.MX_SCAN_SAMPLES} samples once before the capture: the first such call allocates")
                 self._owner = torch.full((self.slots,), -1, dtype=torch.int32, device=device)
-            _capi.check(_capi.load().tlb_mx_write(C.byref(self._struct()), index.data_ptr(), n, x.data_ptr(), dt,
+            _capi.check(_capi.load().tlb_mx_write(self._struct(), index.data_ptr(), n, x.data_ptr(), dt,
                                                   x.stride(1), x.stride(0), None if lengths is None else lengths.data_ptr(),
                                                   handle))
 
@@ -451,7 +469,7 @@ class MxCache:
         with _on(device, stream) as handle:
             out = _out(out, (n, self.tokens, self.cols), dtype, device)
             lengths = None if self.lengths is None else torch.empty(n, dtype=torch.int32, device=device)
-            _capi.check(_capi.load().tlb_mx_read(C.byref(self._struct()), at, n, out.data_ptr(), dt,
+            _capi.check(_capi.load().tlb_mx_read(self._struct(), at, n, out.data_ptr(), dt,
                                                  None if lengths is None else lengths.data_ptr(), handle))
         return out if lengths is None else (out, lengths)
 
@@ -464,7 +482,7 @@ class MxCache:
             codes = torch.empty((n, self.tokens, self.codes.shape[2]), dtype=torch.uint8, device=device)
             scales = torch.empty((n, self.tokens, self.scales.shape[2]), dtype=torch.uint8, device=device)
             lengths = None if self.lengths is None else torch.empty(n, dtype=torch.int32, device=device)
-            _capi.check(_capi.load().tlb_mx_read_codes(C.byref(self._struct()), at, n, codes.data_ptr(), scales.data_ptr(),
+            _capi.check(_capi.load().tlb_mx_read_codes(self._struct(), at, n, codes.data_ptr(), scales.data_ptr(),
                                                        None if lengths is None else lengths.data_ptr(), handle))
-        q = MxTensor(codes, scales, (n, self.tokens, self.cols), self.format, scale=self.scale)
+        q = MxTensor._made(codes, scales, (n, self.tokens, self.cols), n * self.tokens, self.format, self._fmt, self.scale)
         return q if lengths is None else (q, lengths)
