@@ -433,14 +433,16 @@ TLB_API int tlb_mx_matmul(const tlb_mx_rows* a, const tlb_mx_rows* b, void* out,
  * Synchronises. */
 TLB_API int tlb_mx_incomplete(uint32_t* count);
 
-/* Gradients of that product with respect to the values of an operand, g (m, n) packed:
- *   transpose = 0: out (m, q.cols) = g * values(q),    q = b (n rows): the gradient of a
- *   transpose = 1: out (n, q.cols) = g^T * values(q),  q = a (m rows): the gradient of b
- * Every value of g enters whole (fp32 as the sum of three bf16 terms, fp16 of two); sums in fp32. */
-TLB_API int64_t tlb_mx_grad_workspace(int32_t g_dtype, int64_t m, int32_t n, const tlb_mx_rows* q, int32_t transpose,
-                                      int32_t out_dtype);
-TLB_API int tlb_mx_grad(const void* g, int32_t g_dtype, int64_t m, int32_t n, const tlb_mx_rows* q, int32_t transpose,
-                        void* out, int32_t out_dtype, void* workspace, int64_t workspace_bytes, void* stream);
+/* Gradients of that product with respect to the values of its operands, g (m, n) packed:
+ *   grad_a (m, cols) = g * values(b)        grad_b (n, cols) = g^T * values(a)
+ * grad_a or grad_b may be NULL (not wanted), and then b or a too.  Every value of g enters whole (fp32 as the
+ * sum of three bf16 terms, fp16 of two); sums in fp32.  workspace as above, tlb_mx_grad_workspace bytes (which
+ * looks at grad_a and grad_b for NULL alone). */
+TLB_API int64_t tlb_mx_grad_workspace(int32_t g_dtype, int64_t m, int64_t n, const tlb_mx_rows* a, const tlb_mx_rows* b,
+                                      const void* grad_a, int32_t grad_a_dtype, const void* grad_b, int32_t grad_b_dtype);
+TLB_API int tlb_mx_grad(const void* g, int32_t g_dtype, int64_t m, int64_t n, const tlb_mx_rows* a, const tlb_mx_rows* b,
+                        void* grad_a, int32_t grad_a_dtype, void* grad_b, int32_t grad_b_dtype, void* workspace,
+                        int64_t workspace_bytes, void* stream);
 
 /* ---- introspection ---------------------------------------------------------------------
  * Launch geometry the fused kernel would use for `desc` (for tests and the

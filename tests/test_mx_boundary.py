@@ -64,8 +64,10 @@ def test_bad_rows_are_refused_everywhere(kw, code):
     assert lib.tlb_mx_matmul(C.byref(q), C.byref(good), x, 0, None, 0, None) == code
     assert lib.tlb_mx_matmul(C.byref(good), C.byref(q), x, 0, None, 0, None) == code
     assert lib.tlb_mx_matmul_workspace(C.byref(q), C.byref(good), 0) == -1
-    assert lib.tlb_mx_grad(x, 0, 8, 8, C.byref(q), 0, x, 0, None, 0, None) == code
-    assert lib.tlb_mx_grad_workspace(0, 8, 8, C.byref(q), 0, 0) == -1
+    for a, b, ga, gb in ((q, None, None, x), (None, q, x, None), (good, q, x, x), (q, good, x, x)):
+        a, b = (None if r is None else C.byref(r) for r in (a, b))
+        assert lib.tlb_mx_grad(x, 0, 8, 8, a, b, ga, 0, gb, 0, None, 0, None) == code
+        assert lib.tlb_mx_grad_workspace(0, 8, 8, a, b, ga, 0, gb, 0) == -1
 
 
 def test_bad_calls_are_refused():
@@ -108,11 +110,20 @@ def test_bad_calls_are_refused():
     assert lib.tlb_mx_matmul(C.byref(q), C.byref(q), None, 0, None, 0, None) == 1
     assert lib.tlb_mx_matmul(C.byref(q), C.byref(q), 0x5000, 5, None, 0, None) == 1
     assert lib.tlb_mx_matmul(C.byref(q), C.byref(_rows(rows=0)), None, 0, None, 0, None) == 0
-    assert lib.tlb_mx_grad(0x5000, 0, 4, 8, C.byref(q), 2, 0x6000, 0, None, 0, None) == 1
-    assert lib.tlb_mx_grad(0x5000, 0, 4, 7, C.byref(q), 0, 0x6000, 0, None, 0, None) == 1  # the sum runs over 7, q has 8 rows
-    assert lib.tlb_mx_grad(0x5000, 0, 7, 4, C.byref(q), 1, 0x6000, 0, None, 0, None) == 1
-    assert lib.tlb_mx_grad(0x5004, 0, 4, 8, C.byref(q), 0, 0x6000, 0, None, 0, None) == 1
-    assert lib.tlb_mx_grad(0x5000, 0, 0, 8, C.byref(q), 0, None, 0, None, 0, None) == 0
+    r = C.byref(q)  # 8 rows
+
+    def grad(g=0x5000, dtype=0, m=8, n=8, a=r, b=r, ga=0x6000, gb=0x7000, da=0, db=0, ws=None, size=0):
+        return lib.tlb_mx_grad(g, dtype, m, n, a, b, ga, da, gb, db, ws, size, None)
+
+    assert grad() == 1 and b"workspace" in lib.tlb_last_error()
+    assert grad(dtype=3) == grad(da=-1) == grad(db=7) == grad(g=None) == grad(g=0x5004) == grad(ga=0x6008) == 1
+    assert grad(m=7) == grad(n=7) == grad(m=-1) == grad(a=None) == grad(b=None) == grad(ga=None, gb=None) == 1
+    assert grad(b=C.byref(_rows(format=2))) == grad(b=C.byref(_rows(cols=32))) == 1
+    assert grad(m=1 << 30, a=C.byref(_rows(rows=1 << 30))) == 7
+    assert grad(m=0, a=None, gb=None) == 0                                            # nothing to write
+    need = lib.tlb_mx_grad_workspace(0, 8, 8, r, r, 0x6000, 0, 0x7000, 0)
+    assert need > lib.tlb_mx_grad_workspace(0, 8, 8, None, r, 0x6000, 0, None, 0) > 0
+    assert grad(ws=0x8000, size=need - 1) == grad(ws=0x8010, size=need) == 1
 
 
 def test_host_tensors_and_unknown_formats_are_refused():

@@ -112,27 +112,34 @@ tlb::MxProduct product_of(const tlb_mx_rows& a, const tlb_mx_rows& b, int out_dt
     return p;
 }
 
-int check_grad(int g_dtype, int64_t m, int32_t n, const tlb_mx_rows* q, int32_t transpose, int32_t out_dtype) {
-    if (int rc = check_rows(q, "q")) return rc;
+// Fills p but for its pointers to g and the workspace; the results' only say which are wanted.
+int check_grad(tlb::MxGrad& p, int g_dtype, int64_t m, int64_t n, const tlb_mx_rows* a, const tlb_mx_rows* b, const void* grad_a, int32_t grad_a_dtype,
+               const void* grad_b, int32_t grad_b_dtype) {
     if (int rc = check_dtype(g_dtype, "g")) return rc;
-    if (int rc = check_dtype(out_dtype, "out")) return rc;
-    if (m < 0 || n < 0) return fail(TLB_ERR_INVALID_ARG, "g is %lld x %d", static_cast<long long>(m), n);
-    if (m > TLB_MX_MAX_ROWS || n > TLB_MX_MAX_COLS) return fail(TLB_ERR_TOO_LARGE, "g: %lld x %d is too large", static_cast<long long>(m), n);
-    if (m > 0x7fffff00ll / 3) return fail(TLB_ERR_TOO_LARGE, "g: %lld rows are too many", static_cast<long long>(m));
-    if (transpose != 0 && transpose != 1) return fail(TLB_ERR_INVALID_ARG, "transpose = %d must be 0 or 1", transpose);
-    if (q->rows != (transpose ? m : n)) return fail(TLB_ERR_INVALID_ARG, "q has %lld rows, the sum runs over %lld", static_cast<long long>(q->rows), static_cast<long long>(transpose ? m : n));
-    return TLB_OK;
-}
-
-tlb::MxGrad grad_of(int g_dtype, int64_t m, int32_t n, const tlb_mx_rows& q, int32_t transpose, int32_t out_dtype) {
-    tlb::MxGrad p{};
+    if (m < 0 || n < 0) return fail(TLB_ERR_INVALID_ARG, "g is %lld x %lld", static_cast<long long>(m), static_cast<long long>(n));
+    if (m > TLB_MX_MAX_ROWS / 2 || n > TLB_MX_MAX_COLS) return fail(TLB_ERR_TOO_LARGE, "g: %lld x %lld is too large", static_cast<long long>(m), static_cast<long long>(n));
+    if (!grad_a && !grad_b) return fail(TLB_ERR_INVALID_ARG, "no gradient is asked for");
+    if (grad_b) {
+        if (int rc = check_rows(a, "a")) return rc;
+        if (int rc = check_dtype(grad_b_dtype, "grad_b")) return rc;
+        if (a->rows != m) return fail(TLB_ERR_INVALID_ARG, "a has %lld rows, g has %lld", static_cast<long long>(a->rows), static_cast<long long>(m));
+        p.a = rows_of(*a);
+    }
+    if (grad_a) {
+        if (int rc = check_rows(b, "b")) return rc;
+        if (int rc = check_dtype(grad_a_dtype, "grad_a")) return rc;
+        if (b->rows != n) return fail(TLB_ERR_INVALID_ARG, "b has %lld rows, g has %lld columns", static_cast<long long>(b->rows), static_cast<long long>(n));
+        p.b = rows_of(*b);
+    }
+    if (grad_a && grad_b && (a->format != b->format || a->cols != b->cols)) return fail(TLB_ERR_INVALID_ARG, "a and b must have the same format and columns");
     p.g_dtype = g_dtype;
     p.m = m;
-    p.n = n;
-    p.transpose = transpose;
-    p.q = rows_of(q);
-    p.out_dtype = out_dtype;
-    return p;
+    p.n = static_cast<int>(n);
+    p.grad_a = const_cast<void*>(grad_a);
+    p.grad_b = const_cast<void*>(grad_b);
+    p.grad_a_dtype = grad_a_dtype;
+    p.grad_b_dtype = grad_b_dtype;
+    return TLB_OK;
 }
 
 }  // namespace
@@ -258,25 +265,25 @@ int tlb_mx_incomplete(uint32_t* count) {
     return TLB_OK;
 }
 
-int64_t tlb_mx_grad_workspace(int32_t g_dtype, int64_t m, int32_t n, const tlb_mx_rows* q, int32_t transpose, int32_t out_dtype) {
-    if (check_grad(g_dtype, m, n, q, transpose, out_dtype)) return -1;
-    return static_cast<int64_t>(tlb::mx_grad_workspace(grad_of(g_dtype, m, n, *q, transpose, out_dtype)));
+int64_t tlb_mx_grad_workspace(int32_t g_dtype, int64_t m, int64_t n, const tlb_mx_rows* a, const tlb_mx_rows* b, const void* grad_a,
+                              int32_t grad_a_dtype, const void* grad_b, int32_t grad_b_dtype) {
+    tlb::MxGrad p{};
+    if (check_grad(p, g_dtype, m, n, a, b, grad_a, grad_a_dtype, grad_b, grad_b_dtype)) return -1;
+    return static_cast<int64_t>(tlb::mx_grad_workspace(p));
 }
 
-int tlb_mx_grad(const void* g, int32_t g_dtype, int64_t m, int32_t n, const tlb_mx_rows* q, int32_t transpose, void* out,
-                int32_t out_dtype, void* workspace, int64_t workspace_bytes, void* stream) {
-    if (int rc = check_grad(g_dtype, m, n, q, transpose, out_dtype)) return rc;
-    if ((transpose ? static_cast<int64_t>(n) : m) == 0) return TLB_OK;
-    if (!out) return fail(TLB_ERR_INVALID_ARG, "out is NULL");
+int tlb_mx_grad(const void* g, int32_t g_dtype, int64_t m, int64_t n, const tlb_mx_rows* a, const tlb_mx_rows* b, void* grad_a,
+                int32_t grad_a_dtype, void* grad_b, int32_t grad_b_dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+    tlb::MxGrad p{};
+    if (int rc = check_grad(p, g_dtype, m, n, a, b, grad_a, grad_a_dtype, grad_b, grad_b_dtype)) return rc;
     if (!g && m > 0 && n > 0) return fail(TLB_ERR_INVALID_ARG, "g is NULL");
-    if (misaligned(out, 16) || misaligned(g, 16)) return fail(TLB_ERR_INVALID_ARG, "g and out need 16-byte alignment");
-    tlb::MxGrad p = grad_of(g_dtype, m, n, *q, transpose, out_dtype);
+    if (misaligned(grad_a, 16) || misaligned(grad_b, 16) || misaligned(g, 16)) return fail(TLB_ERR_INVALID_ARG, "g, grad_a and grad_b need 16-byte alignment");
     const int64_t need = static_cast<int64_t>(tlb::mx_grad_workspace(p));
     if (need > 0 && (!workspace || workspace_bytes < need || misaligned(workspace, 256)))
         return fail(TLB_ERR_INVALID_ARG, "workspace of %lld bytes (256-byte aligned) is needed", static_cast<long long>(need));
+    if ((!grad_a || m == 0) && (!grad_b || n == 0)) return TLB_OK;
     if (int rc = need_device()) return rc;
     p.g = g;
-    p.out = out;
     p.workspace = workspace;
     if (int e = tlb::launch_mx_grad(p, stream)) return cuda_fail(e, "mx_grad");
     return TLB_OK;

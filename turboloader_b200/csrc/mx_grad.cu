@@ -1,16 +1,19 @@
-// Gradients of the microscaled product: out = alpha * op(g) * values(q), fp32 sums.
-//   transpose = 0:  out (m, cols), sums over n: the gradient of the left operand (q: the right one, n rows)
-//   transpose = 1:  out (n, cols), sums over m: the gradient of the right operand (q: the left one, m rows)
+// Gradients of the microscaled product a * b^T, g (m, n) its result's gradient, fp32 sums:
+//   of a:  out (m, cols) = g * values(b), sums over n          of b:  out (n, cols) = g^T * values(a), sums over m
 //
-// Both are products of bf16 matrices on the tensor cores.  code * block scale has at most 8 significant
-// bits, so widen_kernel writes q's values as bf16 without a rounding (the tensor's scale is alpha).  g enters
-// whole too: bf16 as it is, fp16 as the sum of 2 and fp32 of 3 bf16 terms of 8 bits each (split_kernel),
-// whose products are summed in the same accumulators, the terms being further stages of the sum.
+// Both are products of bf16 matrices on the tensor cores.  code * block scale has at most 8 significant bits, so
+// operands_kernel writes the values as bf16 without a rounding (the tensor's scale is alpha).  g enters whole
+// too: bf16 as it is, fp16 as the sum of 2 and fp32 of 3 bf16 terms of 8 bits each, whose products are summed in
+// the same accumulators, the terms being further stages of the sum.
 //
 // grad_kernel: a pair of CTAs (a cluster of 2) makes output tiles of 256 x tile_n, 64 of the sum a stage.
-// values(q), and g where it is transposed, lie with the sum across the rows: the instructions read them so
+// The values, and g where it is transposed, lie with the sum across the rows: the instructions read them so
 // (the operand's other major order), 64 columns of 64 rows a box.  Roles of the warps as in the product:
 //   warp 0 copies, warp 1 (leader) issues, warps 4-11 write results while the next tile is being summed.
+// The tensor cores cut where they add to an accumulator, about 1e-8 of a sum for every 16 of its terms.  That
+// is below the rounding of a 16-bit result; a result of 32 bits (EXACT) takes the accumulators out every
+// kExactStages stages and adds them in registers, rounding to nearest (12544 x 1000 x 1024, g fp32: 7.4e-6 off
+// without it, EXACTERR with it).
 // With few tiles and a long sum, the sum is split; the parts go to a workspace in fp32 and add_kernel adds
 // them in order, so that the result does not depend on which part ends first.
 #include <atomic>
@@ -26,6 +29,7 @@ constexpr int kSmem = 1024 + kStages * kStageBytes + 8 * kStaging;
 constexpr int kThreads = 384, kPairs = kSms / 2;
 static_assert(kSmem <= 227 * 1024 - 512, "shared memory");
 constexpr unsigned kTmemColumns = 512;
+constexpr int kExactStages = 8;
 
 __device__ unsigned g_gave_up;
 
@@ -38,6 +42,7 @@ struct GradParams {
     long long sum;            // length of the sum, and stages of one term of it
     int term_stages, stages;  // stages: terms * term_stages
     int tile_n, m_tiles, n_tiles, splits;
+    int hold;                 // stages that an accumulator holds at most
     int transpose, scaled, vec_ok;
 };
 
@@ -61,7 +66,7 @@ struct Item {
     }
 };
 
-template <typename T>
+template <typename T, bool EXACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_kernel(const __grid_constant__ GradParams gp) {
     extern __shared__ unsigned char raw[];
     __shared__ unsigned long long bars[2 * kStages + 4];
@@ -95,6 +100,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
     tc_fence_after();
     const unsigned tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
     volatile int* stop = &gave_up;
+    wait_for_previous();
     const int b_boxes = gp.tile_n / 128;  // boxes of 64 columns that this CTA's half of B takes
 
     if (warp == 0) {
@@ -144,26 +150,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
         Ring r;
         unsigned count = 0;
         bool ok = true;
-        for (int it = first_item; ok && it < items; it += step, ++count) {
+        for (int it = first_item; ok && it < items; it += step) {
             const Item item(gp, it);
-            const unsigned buf = count & 1;
-            if (!mbar_wait(acc_empty + 8 * buf, ((count >> 1) & 1) ^ 1, stop)) break;
-            tc_fence_after();
-            const unsigned d = tmem + buf * 256;
-            for (int kt = item.first; kt < item.last; ++kt) {
-                ok = mbar_wait(full + 8 * r.s, r.parity, stop);
+            for (int from = item.first; ok && from < item.last; from += gp.hold, ++count) {
+                const unsigned buf = count & 1;
+                ok = mbar_wait(acc_empty + 8 * buf, ((count >> 1) & 1) ^ 1, stop);
                 if (!ok) break;
                 tc_fence_after();
-                const unsigned a = smem + r.s * kStageBytes, b = a + kStageA;
-                const unsigned long long da = gp.transpose ? smem_desc(a, 8192, 1024, 2) : smem_desc(a, 16, 1024, 2), db = smem_desc(b, 8192, 1024, 2);
-                if (issue) {
+                const unsigned d = tmem + buf * 256;
+                const int to = min(from + gp.hold, item.last);
+                for (int kt = from; kt < to; ++kt) {
+                    ok = mbar_wait(full + 8 * r.s, r.parity, stop);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const unsigned a = smem + r.s * kStageBytes, b = a + kStageA;
+                    const unsigned long long da = gp.transpose ? smem_desc(a, 8192, 1024, 2) : smem_desc(a, 16, 1024, 2), db = smem_desc(b, 8192, 1024, 2);
+                    if (issue) {
 #pragma unroll
-                    for (int i = 0; i < kDepth / 16; ++i) mma_bf16(d, da + i * a_step, db + i * (2048 >> 4), idesc, kt > item.first || i > 0);
-                    tc_commit(empty + 8 * r.s);
-                    if (kt == item.last - 1) tc_commit(acc_full + 8 * buf);
+                        for (int i = 0; i < kDepth / 16; ++i) mma_bf16(d, da + i * a_step, db + i * (2048 >> 4), idesc, kt > from || i > 0);
+                        tc_commit(empty + 8 * r.s);
+                        if (kt == to - 1) tc_commit(acc_full + 8 * buf);
+                    }
+                    __syncwarp();
+                    r.next(kStages);
                 }
-                __syncwarp();
-                r.next(kStages);
             }
         }
     } else if (warp >= 4) {
@@ -172,16 +182,54 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
         const float alpha = gp.scaled ? mx_tensor_scale(gp.q) : 1.0f;
         const unsigned acc_empty_at = at_leader(acc_empty);
         unsigned count = 0;
-        for (int it = first_item; it < items; it += step, ++count) {
+        const unsigned lanes = tmem + (static_cast<unsigned>(quarter * 32) << 16);
+        bool ok = true;
+        for (int it = first_item; ok && it < items; it += step) {
             const Item item(gp, it);
-            const unsigned buf = count & 1;
-            if (!mbar_wait(acc_full + 8 * buf, (count >> 1) & 1, stop)) break;
-            tc_fence_after();
             const long long in_part = static_cast<long long>(2 * item.m + rank) * kTileM + quarter * 32;
             const int n0 = item.n * gp.tile_n;
             const TileOut<T> to{&gp.map_out, static_cast<T*>(gp.out), gp.pitch, item.split * (static_cast<long long>(gp.m_tiles) * 2 * kTileM) + in_part,
                                 gp.splits > 1 ? 32 : static_cast<int>(min(32ll, gp.rows - in_part)), n0, min(gp.tile_n, gp.cols - n0), gp.vec_ok};
-            write_tile(to, tmem + (static_cast<unsigned>(quarter * 32) << 16) + buf * 256, gp.tile_n, half, lane, staging, alpha, acc_empty_at + 8 * buf);
+            if constexpr (!EXACT) {
+                const unsigned buf = count & 1;
+                ok = mbar_wait(acc_full + 8 * buf, (count >> 1) & 1, stop);
+                if (!ok) break;
+                tc_fence_after();
+                write_tile(to, lanes + buf * 256, gp.tile_n, half, lane, staging, alpha, acc_empty_at + 8 * buf);
+                ++count;
+            } else {
+                float sum[4][32];  // this warp's chunks, columns 32 half + 64 i ...
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) sum[i][c] = 0.0f;
+                for (int from = item.first; from < item.last; from += gp.hold, ++count) {
+                    const unsigned buf = count & 1;
+                    ok = mbar_wait(acc_full + 8 * buf, (count >> 1) & 1, stop);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int c0 = half * 32 + i * 64;
+                        if (c0 >= gp.tile_n) continue;
+#pragma unroll
+                        for (int g = 0; g < 2; ++g) {
+                            unsigned v[16];
+                            tmem_load16(lanes + buf * 256 + c0 + g * 16, v);
+                            tmem_load_wait();
+#pragma unroll
+                            for (int c = 0; c < 16; ++c) sum[i][g * 16 + c] = __fadd_rn(sum[i][g * 16 + c], __uint_as_float(v[c]));
+                        }
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_at(acc_empty_at + 8 * buf);
+                }
+                if (!ok) break;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (half * 32 + i * 64 < gp.tile_n) write_chunk(to, sum[i], half * 32 + i * 64, gp.tile_n, lane, staging, alpha);
+            }
         }
         if (lane == 0) tma_store_wait_read();
     }
@@ -195,62 +243,113 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
 }
 
 // ---- operands --------------------------------------------------------------------------------------------------
-// q's values without the tensor's scale, bf16, rows of `pitch` elements; 8 values a thread.
-template <int FMT>
-__global__ void __launch_bounds__(256) widen_kernel(MxRows q, __nv_bfloat16* out, int pitch) {
-    const int units = mx_padded(q.cols) / 8;
-    const long long total = q.rows * units;
-    for (long long u = blockIdx.x * 256ll + threadIdx.x; u < total; u += gridDim.x * 256ll) {
-        const long long row = u / units;
-        const int unit = static_cast<int>(u - row * units);
-        const unsigned char* cp = q.codes + row * mx_code_pitch(FMT, q.cols);
-        const float s = scale_value<FMT>(q.scales[row * mx_scale_pitch(FMT, q.cols) + unit * 8 / mx_block(FMT)]);
-        float v[8];
-        if (FMT == kMxfp8) {
-            const uint2 c = __ldg(reinterpret_cast<const uint2*>(cp) + unit);
-            e4m3_values(c.x, v);
-            e4m3_values(c.y, v + 4);
-        } else {
-            e2m1_values(__ldg(reinterpret_cast<const unsigned*>(cp) + unit), v);
-        }
-        __nv_bfloat162 o[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = __floats2bfloat162_rn(__fmul_rn(v[2 * i], s), __fmul_rn(v[2 * i + 1], s));
-        *reinterpret_cast<uint4*>(out + row * pitch + unit * 8) = *reinterpret_cast<const uint4*>(o);
-    }
+// Values without the tensor's scale, bf16, rows of `pitch` elements (a multiple of 128); 8 values a thread.
+struct Widen {
+    MxRows q;
+    __nv_bfloat16* out;
+    int pitch;
+    long long units;  // of 8 values
+};
+// g as `terms` matrices of bf16, rows of `pitch` elements: each term takes the 8 leading bits of what is left; 8
+// values a thread.
+struct Split {
+    const void* g;
+    int dtype, terms, cols, pitch;
+    long long rows, units;
+    __nv_bfloat16* out;
+};
+
+__device__ __forceinline__ long long quick_div(long long n, int d) {
+    return (n >> 32) == 0 ? static_cast<long long>(static_cast<unsigned>(n) / static_cast<unsigned>(d)) : n / d;
 }
 
-// g as TERMS matrices of bf16, rows of `pitch` elements: each term takes the 8 leading bits of what is left.
-template <typename T, int TERMS>
-__global__ void __launch_bounds__(256) split_kernel(const T* g, long long rows, int cols, __nv_bfloat16* out, int pitch) {
-    const long long total = rows * pitch;
-    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-        const long long row = i / pitch;
-        const int c = static_cast<int>(i - row * pitch);
-        float left = c < cols ? to_float<T>(g[row * cols + c]) : 0.0f;
+template <int FMT>
+__device__ __forceinline__ void widen(const Widen& w, long long u) {
+    const int per_row = w.pitch / 8;
+    const long long row = quick_div(u, per_row);
+    const int unit = static_cast<int>(u - row * per_row);
+    const unsigned char* cp = w.q.codes + row * mx_code_pitch(FMT, w.q.cols);
+    const float s = scale_value<FMT>(w.q.scales[row * mx_scale_pitch(FMT, w.q.cols) + unit * 8 / mx_block(FMT)]);
+    float v[8];
+    if (FMT == kMxfp8) {
+        const uint2 c = __ldg(reinterpret_cast<const uint2*>(cp) + unit);
+        e4m3_values(c.x, v);
+        e4m3_values(c.y, v + 4);
+    } else {
+        e2m1_values(__ldg(reinterpret_cast<const unsigned*>(cp) + unit), v);
+    }
+    __nv_bfloat162 o[4];
 #pragma unroll
-        for (int t = 0; t < TERMS; ++t) {
-            unsigned bits = __float_as_uint(left);
+    for (int i = 0; i < 4; ++i) o[i] = __floats2bfloat162_rn(__fmul_rn(v[2 * i], s), __fmul_rn(v[2 * i + 1], s));
+    *reinterpret_cast<uint4*>(w.out + row * w.pitch + unit * 8) = *reinterpret_cast<const uint4*>(o);
+}
+
+__device__ __forceinline__ void split(const Split& p, long long u) {
+    const int per_row = p.pitch / 8;
+    const long long row = quick_div(u, per_row);
+    const int c0 = static_cast<int>(u - row * per_row) * 8;
+    float left[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const long long at = row * p.cols + c0 + i;
+        left[i] = c0 + i >= p.cols  ? 0.0f
+                  : p.dtype == kF32 ? __ldg(static_cast<const float*>(p.g) + at)
+                  : p.dtype == kF16 ? __half2float(static_cast<const __half*>(p.g)[at])
+                                    : __bfloat162float(static_cast<const __nv_bfloat16*>(p.g)[at]);
+    }
+    for (int t = 0; t < p.terms; ++t) {
+        unsigned short o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            unsigned bits = __float_as_uint(left[i]);
             if ((bits & 0x7fffffffu) > kInfBits) bits |= 0x00400000u;  // a NaN stays one
             bits &= 0xffff0000u;
-            reinterpret_cast<unsigned short*>(out)[t * total + i] = static_cast<unsigned short>(bits >> 16);
+            o[i] = static_cast<unsigned short>(bits >> 16);
             // an infinity or a NaN is whole in the first term
-            left = (bits & 0x7fffffffu) >= kInfBits ? 0.0f : __fsub_rn(left, __uint_as_float(bits));
+            left[i] = (bits & 0x7fffffffu) >= kInfBits ? 0.0f : __fsub_rn(left[i], __uint_as_float(bits));
         }
+        *reinterpret_cast<uint4*>(p.out + (t * p.rows + row) * p.pitch + c0) = *reinterpret_cast<const uint4*>(o);
     }
 }
 
-// The parts of a split sum, added in order.
-template <typename T>
+// All operands of a call at once: units of a, of b, of g.
+template <int FMT>
+__global__ void __launch_bounds__(256) operands_kernel(Widen a, Widen b, Split g) {
+    let_next_start();
+    const long long total = a.units + b.units + g.units;
+    for (long long u = blockIdx.x * 256ll + threadIdx.x; u < total; u += gridDim.x * 256ll) {
+        if (u < a.units) widen<FMT>(a, u);
+        else if (u - a.units < b.units) widen<FMT>(b, u - a.units);
+        else split(g, u - a.units - b.units);
+    }
+}
+
+// The parts of a split sum, added in order; 4 values a thread where rows are whole pieces of 4.
+template <typename T, int N>
 __global__ void __launch_bounds__(256) add_kernel(GradParams gp, const float* parts, long long part, int part_pitch, T* out) {
     const float alpha = mx_tensor_scale(gp.q);
-    const long long total = gp.rows * gp.cols;
+    const int per_row = gp.cols / N;
+    const long long total = gp.rows * per_row;
     for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-        const long long row = i / gp.cols;
-        const float* p = parts + row * part_pitch + (i - row * gp.cols);
-        float v = p[0];
-        for (int s = 1; s < gp.splits; ++s) v = __fadd_rn(v, p[s * part]);
-        out[i] = from_float<T>(__fmul_rn(v, alpha));
+        const long long row = quick_div(i, per_row);
+        const int c = static_cast<int>(i - row * per_row) * N;
+        const float* p = parts + row * part_pitch + c;
+        float v[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = 0.0f;
+        for (int s = 0; s < gp.splits; ++s) {
+            float w[N];
+            if constexpr (N == 4) *reinterpret_cast<float4*>(w) = *reinterpret_cast<const float4*>(p + s * part);
+            else w[0] = p[s * part];
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[j] = s == 0 ? w[j] : __fadd_rn(v[j], w[j]);
+        }
+        __align__(16) T o[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) o[j] = from_float<T>(__fmul_rn(v[j], alpha));
+        if constexpr (N == 4 && sizeof(T) == 4) *reinterpret_cast<float4*>(out + row * gp.cols + c) = *reinterpret_cast<const float4*>(o);
+        else if constexpr (N == 4) *reinterpret_cast<uint2*>(out + row * gp.cols + c) = *reinterpret_cast<const uint2*>(o);
+        else out[row * gp.cols + c] = o[0];
     }
 }
 
@@ -267,121 +366,137 @@ unsigned blocks(long long threads) {
 }
 
 // ---- the host's plan, a function of sizes and types alone ---------------------------------------------------------
-struct Plan {
-    int terms, g_pitch, v_pitch, part_pitch;  // elements
-    bool copy_g;                              // g goes through split_kernel
-    size_t v_bytes, g_bytes, part_bytes;
-    GradParams gp;
-};
-
 size_t round_256(size_t n) { return (n + 255) / 256 * 256; }
 
-Plan plan(const MxGrad& p) {
-    Plan pl{};
-    GradParams& gp = pl.gp;
-    gp.q = p.q;
-    gp.rows = p.transpose ? p.n : p.m;
-    gp.sum = p.transpose ? p.m : p.n;
-    gp.cols = p.q.cols;
-    gp.transpose = p.transpose;
-    pl.terms = p.g_dtype == kBf16 ? 1 : p.g_dtype == kF16 ? 2 : 3;
-    pl.copy_g = pl.terms > 1 || p.n % 8 != 0;
-    pl.g_pitch = (p.n + 7) / 8 * 8;
-    pl.v_pitch = mx_padded(p.q.cols);
+int terms_of(int dtype) { return dtype == kBf16 ? 1 : dtype == kF16 ? 2 : 3; }
+
+struct Shared {  // what both gradients read
+    int terms, g_pitch;
+    bool copy_g;
+    size_t g_bytes, a_bytes, b_bytes;  // 0: not needed
+};
+
+Shared shared_of(const MxGrad& p) {
+    Shared s{};
+    s.terms = terms_of(p.g_dtype);
+    s.copy_g = s.terms > 1 || p.n % 8 != 0;
+    s.g_pitch = (p.n + 7) / 8 * 8;
+    s.g_bytes = s.copy_g ? round_256(static_cast<size_t>(s.terms) * p.m * s.g_pitch * 2) : 0;
+    s.a_bytes = p.grad_b ? round_256(static_cast<size_t>(p.m) * mx_padded(p.a.cols) * 2) : 0;
+    s.b_bytes = p.grad_a ? round_256(static_cast<size_t>(p.n) * mx_padded(p.b.cols) * 2) : 0;
+    return s;
+}
+
+// of_b: the gradient of b, which is transposed.
+GradParams plan(const MxGrad& p, const Shared& sh, bool of_b) {
+    GradParams gp{};
+    gp.q = of_b ? p.a : p.b;
+    gp.rows = of_b ? p.n : p.m;
+    gp.sum = of_b ? p.m : p.n;
+    gp.cols = gp.q.cols;
+    gp.transpose = of_b;
     gp.term_stages = static_cast<int>((gp.sum + kDepth - 1) / kDepth);
-    gp.stages = pl.terms * gp.term_stages;
+    gp.stages = sh.terms * gp.term_stages;
     gp.m_tiles = static_cast<int>((gp.rows + 2 * kTileM - 1) / (2 * kTileM));
     // Two widths; the wider copies less for each product.  And the sum in as many parts as leave no pair idle, each of
-    // 16 stages at least (a part costs its writing and reading again).
+    // 16 stages at least; writing and adding the parts costs as much as some 24 stages.
     long long best = 0;
     for (int w = 128; w <= 256; w += 128) {
         const long long n_tiles = (gp.cols + w - 1) / w, tiles = gp.m_tiles * n_tiles;
         const long long most = tiles >= kPairs ? 1 : kPairs / tiles, long_enough = gp.stages / 16 > 0 ? gp.stages / 16 : 1;
-        const long long splits = most < long_enough ? most : long_enough;
-        const long long cost = (tiles * splits + kPairs - 1) / kPairs * ((gp.stages + splits - 1) / splits) * (w + 64);
-        if (best == 0 || cost < best) {
-            best = cost;
-            gp.tile_n = w;
-            gp.n_tiles = static_cast<int>(n_tiles);
-            gp.splits = static_cast<int>(splits);
+        for (long long splits = most < long_enough ? most : long_enough;; splits = 1) {
+            const long long cost = (tiles * splits + kPairs - 1) / kPairs * ((gp.stages + splits - 1) / splits + (splits > 1 ? 24 : 4)) * (w + 64);
+            if (best == 0 || cost < best) {
+                best = cost;
+                gp.tile_n = w;
+                gp.n_tiles = static_cast<int>(n_tiles);
+                gp.splits = static_cast<int>(splits);
+            }
+            if (splits == 1) break;
         }
     }
-    pl.v_bytes = round_256(static_cast<size_t>(p.q.rows) * pl.v_pitch * 2);
-    pl.g_bytes = pl.copy_g ? round_256(static_cast<size_t>(pl.terms) * p.m * pl.g_pitch * 2) : 0;
-    pl.part_pitch = gp.n_tiles * gp.tile_n;
-    pl.part_bytes = gp.splits > 1 ? static_cast<size_t>(gp.splits) * gp.m_tiles * 2 * kTileM * pl.part_pitch * 4 : 0;
-    return pl;
+    gp.hold = (of_b ? p.grad_b_dtype : p.grad_a_dtype) == kF32 ? kExactStages : gp.stages;
+    return gp;
 }
 
-template <typename T>
-int launch_grad(const GradParams& gp, cudaStream_t st) {
+int part_pitch(const GradParams& gp) { return gp.n_tiles * gp.tile_n; }
+size_t part_bytes(const GradParams& gp) {
+    return gp.splits > 1 ? static_cast<size_t>(gp.splits) * gp.m_tiles * 2 * kTileM * part_pitch(gp) * 4 : 0;
+}
+
+template <typename T, bool EXACT>
+int launch_grad(const GradParams& gp, cudaStream_t st, bool after_operands) {
     static std::atomic<unsigned long long> prepared{0};  // one bit a device
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return last_error();
     const unsigned long long bit = 1ull << (dev & 63);
     if (!(prepared.load(std::memory_order_acquire) & bit)) {
-        const cudaError_t e = cudaFuncSetAttribute(grad_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+        const cudaError_t e = cudaFuncSetAttribute(grad_kernel<T, EXACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
         if (e != cudaSuccess) return static_cast<int>(e);
         prepared.fetch_or(bit, std::memory_order_release);
     }
     const int items = gp.m_tiles * gp.n_tiles * gp.splits;
-    grad_kernel<T><<<2 * (items < kPairs ? items : kPairs), kThreads, kSmem, st>>>(gp);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(2 * (items < kPairs ? items : kPairs)));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // set up while operands_kernel runs
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = after_operands ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, grad_kernel<T, EXACT>, gp);
+    if (e != cudaSuccess) return static_cast<int>(e);
     mx_count_launch();
     return last_error();
 }
 
+// g: its terms, rows of g_pitch elements; values: of the other operand; parts: workspace of a split sum.
 template <typename T>
-int launch_typed(const MxGrad& p, Plan& pl, cudaStream_t st) {
-    GradParams& gp = pl.gp;
+int one_grad(const MxGrad& p, const Shared& sh, bool of_b, const void* g, const void* values, void* parts, void* result, bool after_operands, cudaStream_t st) {
+    GradParams gp = plan(p, sh, of_b);
+    if (gp.rows == 0) return 0;
     if (gp.sum == 0) {
-        zero_kernel<T><<<blocks(gp.rows * gp.cols), 256, 0, st>>>(static_cast<T*>(p.out), gp.rows * gp.cols);
+        zero_kernel<T><<<blocks(gp.rows * gp.cols), 256, 0, st>>>(static_cast<T*>(result), gp.rows * gp.cols);
         mx_count_launch();
         return last_error();
     }
-    unsigned char* ws = static_cast<unsigned char*>(p.workspace);
-    __nv_bfloat16* v = reinterpret_cast<__nv_bfloat16*>(ws);
-    const unsigned widen_blocks = blocks(p.q.rows * (pl.v_pitch / 8));
-    if (p.q.format == kNvfp4) widen_kernel<kNvfp4><<<widen_blocks, 256, 0, st>>>(p.q, v, pl.v_pitch);
-    else if (p.q.format == kMxfp4) widen_kernel<kMxfp4><<<widen_blocks, 256, 0, st>>>(p.q, v, pl.v_pitch);
-    else widen_kernel<kMxfp8><<<widen_blocks, 256, 0, st>>>(p.q, v, pl.v_pitch);
-    mx_count_launch();
-    const void* g = p.g;
-    if (pl.copy_g) {
-        __nv_bfloat16* terms = reinterpret_cast<__nv_bfloat16*>(ws + pl.v_bytes);
-        const unsigned n = blocks(p.m * pl.g_pitch);
-        if (p.g_dtype == kF32) split_kernel<float, 3><<<n, 256, 0, st>>>(static_cast<const float*>(p.g), p.m, p.n, terms, pl.g_pitch);
-        else if (p.g_dtype == kF16) split_kernel<__half, 2><<<n, 256, 0, st>>>(static_cast<const __half*>(p.g), p.m, p.n, terms, pl.g_pitch);
-        else split_kernel<__nv_bfloat16, 1><<<n, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(p.g), p.m, p.n, terms, pl.g_pitch);
-        mx_count_launch();
-        g = terms;
-    }
-    if (int e = last_error()) return e;
-    const unsigned long long g_rows = static_cast<unsigned long long>(pl.terms) * p.m;
-    if (int e = mx_encode_map(&gp.map_a, 2, g, p.n, g_rows, pl.g_pitch * 2ull, 64, gp.transpose ? kDepth : kTileM, 1)) return e;
-    if (int e = mx_encode_map(&gp.map_b, 2, v, p.q.cols, p.q.rows, pl.v_pitch * 2ull, 64, kDepth, 1)) return e;
+    const unsigned long long g_rows = static_cast<unsigned long long>(sh.terms) * p.m;
+    if (int e = mx_encode_map(&gp.map_a, 2, g, p.n, g_rows, sh.g_pitch * 2ull, 64, gp.transpose ? kDepth : kTileM, 1)) return e;
+    if (int e = mx_encode_map(&gp.map_b, 2, values, gp.cols, gp.q.rows, mx_padded(gp.cols) * 2ull, 64, kDepth, 1)) return e;
     if (gp.splits > 1) {
-        float* parts = reinterpret_cast<float*>(ws + pl.v_bytes + pl.g_bytes);
-        const unsigned long long part_rows = static_cast<unsigned long long>(gp.m_tiles) * 2 * kTileM;
+        const unsigned long long part_rows = static_cast<unsigned long long>(gp.m_tiles) * 2 * kTileM, row_bytes = static_cast<unsigned long long>(part_pitch(gp)) * 4;
         gp.out = parts;
-        gp.pitch = pl.part_pitch;
+        gp.pitch = part_pitch(gp);
         gp.scaled = 0;
         gp.vec_ok = 1;
-        const unsigned long long row_bytes = static_cast<unsigned long long>(pl.part_pitch) * 4;
         if (int e = mx_encode_map(&gp.map_out, 1, parts, row_bytes, gp.splits * part_rows, row_bytes, 128, 32, 1)) return e;
-        if (int e = launch_grad<float>(gp, st)) return e;
-        add_kernel<T><<<blocks(gp.rows * gp.cols), 256, 0, st>>>(gp, parts, static_cast<long long>(part_rows) * pl.part_pitch, pl.part_pitch,
-                                                                 static_cast<T*>(p.out));
+        if (int e = sizeof(T) == 4 ? launch_grad<float, true>(gp, st, after_operands) : launch_grad<float, false>(gp, st, after_operands)) return e;
+        const long long part = static_cast<long long>(part_rows) * part_pitch(gp);
+        if (gp.cols % 4 == 0)
+            add_kernel<T, 4><<<blocks(gp.rows * (gp.cols / 4)), 256, 0, st>>>(gp, static_cast<const float*>(parts), part, part_pitch(gp), static_cast<T*>(result));
+        else
+            add_kernel<T, 1><<<blocks(gp.rows * gp.cols), 256, 0, st>>>(gp, static_cast<const float*>(parts), part, part_pitch(gp), static_cast<T*>(result));
         mx_count_launch();
         return last_error();
     }
-    gp.out = p.out;
+    gp.out = result;
     gp.pitch = gp.cols;
     gp.scaled = 1;
     const unsigned long long row_bytes = static_cast<unsigned long long>(gp.cols) * sizeof(T);
     gp.vec_ok = row_bytes % 16 == 0;
     if (gp.vec_ok)
-        if (int e = mx_encode_map(&gp.map_out, 1, p.out, row_bytes, gp.rows, row_bytes, 128, 32, 1)) return e;
-    return launch_grad<T>(gp, st);
+        if (int e = mx_encode_map(&gp.map_out, 1, result, row_bytes, gp.rows, row_bytes, 128, 32, 1)) return e;
+    return launch_grad<T, sizeof(T) == 4>(gp, st, after_operands);
+}
+
+int typed_grad(const MxGrad& p, const Shared& sh, bool of_b, const void* g, const void* values, void* parts, bool after_operands, cudaStream_t st) {
+    const int dtype = of_b ? p.grad_b_dtype : p.grad_a_dtype;
+    void* result = of_b ? p.grad_b : p.grad_a;
+    if (dtype == kF32) return one_grad<float>(p, sh, of_b, g, values, parts, result, after_operands, st);
+    if (dtype == kBf16) return one_grad<__nv_bfloat16>(p, sh, of_b, g, values, parts, result, after_operands, st);
+    return one_grad<__half>(p, sh, of_b, g, values, parts, result, after_operands, st);
 }
 
 }  // namespace
@@ -390,16 +505,36 @@ int mx_grad_gave_up(unsigned* count) { return static_cast<int>(cudaMemcpyFromSym
 
 size_t mx_grad_workspace(const MxGrad& p) {
     if (p.m == 0 || p.n == 0) return 0;
-    const Plan pl = plan(p);
-    return pl.v_bytes + pl.g_bytes + pl.part_bytes;
+    const Shared sh = shared_of(p);
+    // the parts of the two, which run one after the other, share their room
+    const size_t of_a = p.grad_a ? part_bytes(plan(p, sh, false)) : 0, of_b = p.grad_b ? part_bytes(plan(p, sh, true)) : 0;
+    return sh.g_bytes + sh.a_bytes + sh.b_bytes + (of_a > of_b ? of_a : of_b);
 }
 
 int launch_mx_grad(const MxGrad& p, void* stream) {
-    Plan pl = plan(p);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (p.out_dtype == kF32) return launch_typed<float>(p, pl, st);
-    if (p.out_dtype == kBf16) return launch_typed<__nv_bfloat16>(p, pl, st);
-    return launch_typed<__half>(p, pl, st);
+    const Shared sh = shared_of(p);
+    unsigned char* ws = static_cast<unsigned char*>(p.workspace);
+    unsigned char *a_at = ws + sh.g_bytes, *b_at = a_at + sh.a_bytes, *parts = b_at + sh.b_bytes;
+    const bool any = p.m > 0 && p.n > 0;
+    if (any) {
+        const Widen a{p.a, reinterpret_cast<__nv_bfloat16*>(a_at), mx_padded(p.a.cols), sh.a_bytes ? p.m * (mx_padded(p.a.cols) / 8) : 0};
+        const Widen b{p.b, reinterpret_cast<__nv_bfloat16*>(b_at), mx_padded(p.b.cols), sh.b_bytes ? static_cast<long long>(p.n) * (mx_padded(p.b.cols) / 8) : 0};
+        const Split g{p.g, p.g_dtype, sh.terms, p.n, sh.g_pitch, p.m, sh.copy_g ? p.m * (sh.g_pitch / 8) : 0, reinterpret_cast<__nv_bfloat16*>(ws)};
+        const unsigned n = blocks(a.units + b.units + g.units);
+        const int format = p.grad_b ? p.a.format : p.b.format;
+        if (format == kNvfp4) operands_kernel<kNvfp4><<<n, 256, 0, st>>>(a, b, g);
+        else if (format == kMxfp4) operands_kernel<kMxfp4><<<n, 256, 0, st>>>(a, b, g);
+        else operands_kernel<kMxfp8><<<n, 256, 0, st>>>(a, b, g);
+        mx_count_launch();
+        if (int e = last_error()) return e;
+    }
+    const void* g = sh.copy_g ? static_cast<const void*>(ws) : p.g;
+    if (p.grad_a)
+        if (int e = typed_grad(p, sh, false, g, b_at, parts, any, st)) return e;
+    if (p.grad_b)
+        if (int e = typed_grad(p, sh, true, g, a_at, parts, any && !p.grad_a, st)) return e;
+    return 0;
 }
 
 }  // namespace tlb

@@ -62,16 +62,16 @@ int mx_gave_up(unsigned* count);  // products and gradients on this device that 
 size_t mx_matmul_workspace(const MxProduct& p);
 int launch_mx_matmul(const MxProduct& p, void* stream);
 
-// out = alpha * op(g) * values(q): op(g) = g (m, n) with q of n rows, or its transpose with q of m rows.
+// Gradients of a * b^T, g (m, n): of a, out (m, cols) = g * values(b), and of b, out (n, cols) = g^T * values(a).
+// grad_a or grad_b nullptr: not wanted, and the other operand not read.
 struct MxGrad {
     const void* g;           // (m, n) packed
     int g_dtype;
     long long m;
     int n;
-    int transpose;           // 0: out (m, cols), sums over n.  1: out (n, cols), sums over m
-    MxRows q;
-    void* out;
-    int out_dtype;
+    MxRows a, b;
+    void *grad_a, *grad_b;   // packed
+    int grad_a_dtype, grad_b_dtype;
     void* workspace;
 };
 // A 2-D tensor map (cuTensorMapEncodeTiled); a cudaError_t value.

@@ -31,13 +31,70 @@ struct TileOut {
     int vec_ok;              // rows are multiples of 16 bytes
 };
 
+// A chunk of 128 bytes of a warp's 32 rows, columns c0 to c0 + 128 / sizeof(T) of the tile, from registers: lane l
+// holds row l.
+template <typename T>
+__device__ __forceinline__ void write_chunk(const TileOut<T>& to, const float* v, int c0, int tile_n, int lane, unsigned staging, float alpha) {
+    constexpr int chunk = 128 / sizeof(T), per = 16 / sizeof(T);  // columns of a chunk, of 16 bytes
+    const int groups = min(chunk, tile_n - c0) / 16;              // of 16 columns
+    const bool whole = to.vec_ok && groups == chunk / 16;
+    if (whole) {
+        if (lane == 0) tma_store_wait_read();
+        __syncwarp();
+    }
+    T o[chunk];
+#pragma unroll
+    for (int i = 0; i < chunk; ++i) o[i] = from_float<T>(__fmul_rn(v[i], alpha));
+    const uint4* pieces = reinterpret_cast<const uint4*>(o);
+    auto stage = [&]() {  // 16-byte pieces in the order of the 128-byte swizzle
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(staging + lane * 128 + ((i ^ (lane & 7)) * 16)), "r"(pieces[i].x),
+                         "r"(pieces[i].y), "r"(pieces[i].z), "r"(pieces[i].w)
+                         : "memory");
+    };
+    if (whole) {
+        stage();
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0 && to.rows > 0 && c0 < to.width)
+            tma_store_2d(to.map, (to.n0 + c0) * static_cast<int>(sizeof(T)), static_cast<int>(to.m0), staging);
+    } else if (to.vec_ok) {  // the tile's last, narrower chunk
+        T* out = to.out + (to.m0 + lane) * to.pitch + to.n0 + c0;
+        if (lane < to.rows) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i * per < groups * 16 && c0 + i * per < to.width) reinterpret_cast<uint4*>(out)[i] = pieces[i];
+        }
+    } else {
+        __syncwarp();
+        stage();
+        __syncwarp();
+        const int cols = min(groups * 16, to.width - c0);
+        T* out = to.out + to.m0 * to.pitch + to.n0 + c0;
+        for (int r = 0; r < to.rows; ++r)
+            for (int c = lane; c < cols; c += 32) {
+                const unsigned at = staging + r * 128 + ((c / per) ^ (r & 7)) * 16 + c % per * static_cast<int>(sizeof(T));
+                if constexpr (sizeof(T) == 4) {
+                    unsigned bits;
+                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(bits) : "r"(at));
+                    reinterpret_cast<unsigned*>(out)[static_cast<long long>(r) * to.pitch + c] = bits;
+                } else {
+                    unsigned short bits;
+                    asm volatile("ld.shared.b16 %0, [%1];" : "=h"(bits) : "r"(at));
+                    reinterpret_cast<unsigned short*>(out)[static_cast<long long>(r) * to.pitch + c] = bits;
+                }
+            }
+    }
+}
+
 // One warp's part of a tile: the 32 rows of its TMEM lanes (`from`: its lane bits and first column), every
 // second chunk of 128 bytes of them, beginning with chunk `half`.  Arrives on `released` (of the leader) once
 // its last columns are in registers, so that the next sums may start before the stores are done.
 template <typename T>
 __device__ __forceinline__ void write_tile(const TileOut<T>& to, unsigned from, int tile_n, int half, int lane, unsigned staging, float alpha,
                                            unsigned released) {
-    constexpr int chunk = 128 / sizeof(T), per = 16 / sizeof(T);  // columns of a chunk, of 16 bytes
+    constexpr int chunk = 128 / sizeof(T);
     auto release = [&]() {
         tc_fence_before();
         __syncwarp();
@@ -45,62 +102,16 @@ __device__ __forceinline__ void write_tile(const TileOut<T>& to, unsigned from, 
     };
     if (half * chunk >= tile_n) release();
     for (int c0 = half * chunk; c0 < tile_n; c0 += 2 * chunk) {
-        const int groups = min(chunk, tile_n - c0) / 16;  // of 16 columns
-        const bool whole = to.vec_ok && groups == chunk / 16;
         unsigned v[chunk];
 #pragma unroll
         for (int g = 0; g < chunk / 16; ++g)
-            if (g < groups) tmem_load16(from + c0 + g * 16, v + 16 * g);
+            if (c0 + g * 16 < tile_n) tmem_load16(from + c0 + g * 16, v + 16 * g);
         tmem_load_wait();
         if (c0 + 2 * chunk >= tile_n) release();
-        if (whole) {
-            if (lane == 0) tma_store_wait_read();
-            __syncwarp();
-        }
-        T o[chunk];
+        float f[chunk];
 #pragma unroll
-        for (int i = 0; i < chunk; ++i) o[i] = from_float<T>(__fmul_rn(__uint_as_float(v[i]), alpha));
-        const uint4* pieces = reinterpret_cast<const uint4*>(o);
-        auto stage = [&]() {  // 16-byte pieces in the order of the 128-byte swizzle
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(staging + lane * 128 + ((i ^ (lane & 7)) * 16)), "r"(pieces[i].x),
-                             "r"(pieces[i].y), "r"(pieces[i].z), "r"(pieces[i].w)
-                             : "memory");
-        };
-        if (whole) {
-            stage();
-            fence_async_shared();
-            __syncwarp();
-            if (lane == 0 && to.rows > 0 && c0 < to.width)
-                tma_store_2d(to.map, (to.n0 + c0) * static_cast<int>(sizeof(T)), static_cast<int>(to.m0), staging);
-        } else if (to.vec_ok) {  // the tile's last, narrower chunk
-            T* out = to.out + (to.m0 + lane) * to.pitch + to.n0 + c0;
-            if (lane < to.rows) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (i * per < groups * 16 && c0 + i * per < to.width) reinterpret_cast<uint4*>(out)[i] = pieces[i];
-            }
-        } else {
-            __syncwarp();
-            stage();
-            __syncwarp();
-            const int cols = min(groups * 16, to.width - c0);
-            T* out = to.out + to.m0 * to.pitch + to.n0 + c0;
-            for (int r = 0; r < to.rows; ++r)
-                for (int c = lane; c < cols; c += 32) {
-                    const unsigned at = staging + r * 128 + ((c / per) ^ (r & 7)) * 16 + c % per * static_cast<int>(sizeof(T));
-                    if constexpr (sizeof(T) == 4) {
-                        unsigned bits;
-                        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(bits) : "r"(at));
-                        reinterpret_cast<unsigned*>(out)[static_cast<long long>(r) * to.pitch + c] = bits;
-                    } else {
-                        unsigned short bits;
-                        asm volatile("ld.shared.b16 %0, [%1];" : "=h"(bits) : "r"(at));
-                        reinterpret_cast<unsigned short*>(out)[static_cast<long long>(r) * to.pitch + c] = bits;
-                    }
-                }
-        }
+        for (int i = 0; i < chunk; ++i) f[i] = __uint_as_float(v[i]);
+        write_chunk(to, f, c0, tile_n, lane, staging, alpha);
     }
 }
 

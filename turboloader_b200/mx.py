@@ -281,20 +281,23 @@ def mx_incomplete() -> int:
     return int(count.value)
 
 
-def _grad(g, q, transpose, dtype):
-    """g (m, n) times values(q) (n, k), or with ``transpose`` g^T times values(q) (m, k); in ``dtype``."""
+def _grads(g, qa, qb, a_dtype, b_dtype):
+    """(grad_a, grad_b) of values(a) @ values(b).T for g (m, n); a dtype of None: not wanted."""
     lib = _capi.load()
     device = g.device
     m, n = g.shape
-    dt, gt = _DTYPES[dtype], _DTYPES[g.dtype]
+    cols = (qa or qb).shape[-1]
+    gt = _DTYPES[g.dtype]
     with _on(device, None) as handle:
-        out = torch.empty((n if transpose else m, q.shape[-1]), dtype=dtype, device=device)
-        sq = q._struct()
-        size = lib.tlb_mx_grad_workspace(gt, m, n, sq, transpose, dt)
+        ga = None if a_dtype is None else torch.empty((m, cols), dtype=a_dtype, device=device)
+        gb = None if b_dtype is None else torch.empty((n, cols), dtype=b_dtype, device=device)
+        # an empty tensor has no address; any other one says that its gradient is wanted
+        at = (None if gb is None else qa._struct(), None if ga is None else qb._struct(), None if ga is None else ga.data_ptr() or 16,
+              _DTYPES.get(a_dtype, 0), None if gb is None else gb.data_ptr() or 16, _DTYPES.get(b_dtype, 0))
+        size = lib.tlb_mx_grad_workspace(gt, m, n, *at)
         ws = _workspace(size, device)
-        _capi.check(lib.tlb_mx_grad(g.data_ptr(), gt, m, n, sq, transpose, out.data_ptr(), dt, None if ws is None else ws.data_ptr(), size,
-                                    handle))
-    return out
+        _capi.check(lib.tlb_mx_grad(g.data_ptr(), gt, m, n, *at, None if ws is None else ws.data_ptr(), size, handle))
+    return ga, gb
 
 
 def _spaced(x):
@@ -335,9 +338,8 @@ class _MxLinear(torch.autograd.Function):
             g = g.reshape(-1, g.shape[-1]).contiguous()
         if g.data_ptr() % 16:
             g = g.clone()
-        gx = _grad(g, qw, 0, ctx.types[0]).view(ctx.x_shape) if qw is not None else None
-        gw = _grad(g, qx, 1, ctx.types[1]) if qx is not None else None
-        return gx, gw, None, None, None, None, None, None
+        gx, gw = _grads(g, qx, qw, *ctx.types)
+        return None if gx is None else gx.view(ctx.x_shape), gw, None, None, None, None, None, None
 
 
 def mx_linear(x, weight, format="nvfp4", *, scale=1.0, weight_scale=1.0, dtype=None):
