@@ -369,7 +369,7 @@ TLB_API void tlb_epoch_destroy(tlb_epoch* e);
  * Layout: rows are padded to 128 values; a row of codes takes tlb_mx_code_pitch bytes (4-bit codes: two a
  * byte, the earlier value in the low half) and a row of scales tlb_mx_scale_pitch bytes, rows packed
  * without gaps.  Pad codes and pad scale bytes are zero (the calls below write them so, and the products
- * rely on it). */
+ * rely on it); an nvfp4 scale byte has no sign. */
 enum { TLB_MX_NVFP4 = 0, TLB_MX_MXFP4 = 1, TLB_MX_MXFP8 = 2 };
 #define TLB_MX_MAX_COLS (1 << 20)
 #define TLB_MX_MAX_ROWS (1ll << 30)
@@ -426,6 +426,12 @@ TLB_API int tlb_mx_read_codes(const tlb_mx_cache* cache, const int64_t* index, i
  * used by this call alone until its work has ended. */
 TLB_API int64_t tlb_mx_matmul_workspace(const tlb_mx_rows* a, const tlb_mx_rows* b, int32_t out_dtype);
 TLB_API int tlb_mx_matmul(const tlb_mx_rows* a, const tlb_mx_rows* b, void* out, int32_t out_dtype, void* workspace,
+                          int64_t workspace_bytes, void* stream);
+
+/* A linear layer: tlb_mx_quantize of x into a and of w into b (each where it is not NULL; else the rows are used
+ * as they are), then tlb_mx_matmul. */
+TLB_API int tlb_mx_linear(const tlb_mx_rows* a, const void* x, int32_t x_dtype, int64_t x_pitch, const tlb_mx_rows* b,
+                          const void* w, int32_t w_dtype, int64_t w_pitch, void* out, int32_t out_dtype, void* workspace,
                           int64_t workspace_bytes, void* stream);
 
 /* Products and gradients on the current device since the library was loaded whose kernels gave up a

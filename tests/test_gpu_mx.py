@@ -331,6 +331,38 @@ def test_gradients_of_mixed_types_held_operands_and_scales():
         assert not tb.mx_linear(held, w, "nvfp4").requires_grad
 
 
+def test_linear_of_nothing():
+    w = torch.randn(5, 40, device="cuda", requires_grad=True)
+    x = torch.randn(0, 40, device="cuda", requires_grad=True)
+    y = tb.mx_linear(x, w, "mxfp4")
+    assert y.shape == (0, 5)
+    gx, gw = torch.autograd.grad(y, [x, w], torch.ones(0, 5, device="cuda"))
+    assert gx.shape == (0, 40) and torch.equal(gw, torch.zeros(5, 40, device="cuda"))
+    w = torch.randn(0, 40, device="cuda", requires_grad=True)
+    x = torch.randn(3, 40, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    y = tb.mx_linear(x, w, "nvfp4")
+    gx, gw = torch.autograd.grad(y, [x, w], torch.ones(3, 0, device="cuda"))
+    assert y.shape == (3, 0) and gw.shape == (0, 40) and torch.equal(gx, torch.zeros_like(x))
+
+
+def test_infinities_and_nan_in_the_gradient_stay_in_their_rows():
+    g = torch.Generator(device="cuda").manual_seed(4)
+    m, n, k = 130, 70, 64
+    for dtype in DTYPES:
+        x = torch.randn(m, k, generator=g, device="cuda").to(dtype).requires_grad_(True)
+        w = torch.randn(n, k, generator=g, device="cuda").to(dtype).requires_grad_(True)
+        clean = torch.randn(m, n, generator=g, device="cuda").to(dtype)
+        dirty = clean.clone()
+        dirty[3, 5], dirty[129, 7] = float("nan"), float("inf")
+        y = tb.mx_linear(x, w, "mxfp8")
+        ax, aw = torch.autograd.grad(y, [x, w], clean, retain_graph=True)
+        bx, bw = torch.autograd.grad(y, [x, w], dirty)
+        assert torch.isnan(bx[3]).all() and not torch.isfinite(bx[129]).any() and torch.isnan(bw[5]).all() and not torch.isfinite(bw[7]).any()
+        rows, cols = torch.ones(m, dtype=torch.bool), torch.ones(n, dtype=torch.bool)
+        rows[[3, 129]], cols[[5, 7]] = False, False
+        assert torch.equal(ax[rows], bx[rows]) and torch.equal(aw[cols], bw[cols])
+
+
 def test_gradients_against_differences():
     """The product is linear in each operand's values: moving one value between two points of its grid, scale
     unchanged, moves the result by the difference times the other operand."""
@@ -429,6 +461,53 @@ def test_captured_and_replayed():
             got = [t.clone() for t in s["out"]]
             for have, want in zip(got, step()):
                 assert torch.equal(have, want)
+
+
+def test_captured_without_a_call_before():
+    """In a fresh process: the first call of each kernel is a captured one."""
+    import subprocess
+    import sys
+
+    code = """if 1:
+        import torch, turboloader_b200 as tb
+        x, w = torch.randn(300, 256, device="cuda"), torch.randn(64, 256, device="cuda")
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            a, b = tb.mx_quantize(x), tb.mx_quantize(w)
+            y, z, v = tb.mx_matmul(a, b, torch.float32), tb.mx_matmul(tb.mx_quantize(x[:1]), b, torch.float32), a.dequantize()
+        graph.replay()
+        torch.cuda.synchronize()
+        a, b = tb.mx_quantize(x), tb.mx_quantize(w)
+        assert torch.equal(y, tb.mx_matmul(a, b, torch.float32)) and torch.equal(v, a.dequantize())
+        assert torch.equal(z, tb.mx_matmul(tb.mx_quantize(x[:1]), b, torch.float32)) and tb.mx_incomplete() == 0
+    """
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300)
+
+
+def test_offsets_beyond_32_bits():
+    """A cache whose codes pass 4 GiB, and a result of more than 2^31 values: their far ends."""
+    slots, tokens, cols = 4100, 256, 4096 + 32
+    cache = tb.MxCache(torch.empty(slots, tokens, 2112, dtype=torch.uint8, device="cuda"), torch.empty(slots, tokens, 132, dtype=torch.uint8, device="cuda"),
+                       cols, "mxfp4")
+    assert cache.codes.numel() == slots * tokens * 2112 > 2 ** 31
+    x = torch.randn(2, tokens, cols, device="cuda")
+    index = torch.tensor([slots - 1, 0], device="cuda")
+    cache.write(index, x)
+    codes, scales = encode(_np(x[0]), "mxfp4")
+    _same(cache.codes[-1].cpu().numpy(), codes[:, :2112])
+    _same(cache.scales[-1].cpu().numpy(), scales[:, :132])
+    want = tb.mx_quantize(x, "mxfp4")
+    assert torch.equal(cache.read(index, torch.float32), want.dequantize())
+    assert torch.equal(cache.read_mx(index).codes.view(-1), want.codes.view(-1))
+    del cache
+    m, n = 300_001, 8192
+    a = tb.mx_quantize(torch.randn(m, 64, device="cuda"), "mxfp4")
+    b = tb.mx_quantize(torch.randn(n, 64, device="cuda"), "mxfp4")
+    y = tb.mx_matmul(a, b)
+    assert y.numel() > 2 ** 31
+    tail = tb.MxTensor(a.codes[m - 300:], a.scales[m - 300:], (300, 64), "mxfp4")
+    assert torch.equal(y[m - 300:], tb.mx_matmul(tail, b))
 
 
 def test_feature_loader_serves_what_was_written():

@@ -212,6 +212,7 @@ def load() -> C.CDLL:
             ("tlb_mx_read_codes", C.c_int, [cache, ptr, i64, ptr, ptr, ptr, ptr]),
             ("tlb_mx_matmul_workspace", i64, [rows, rows, i32]),
             ("tlb_mx_matmul", C.c_int, [rows, rows, ptr, i32, ptr, i64, ptr]),
+            ("tlb_mx_linear", C.c_int, [rows, ptr, i32, i64, rows, ptr, i32, i64, ptr, i32, ptr, i64, ptr]),
             ("tlb_mx_incomplete", C.c_int, [C.POINTER(C.c_uint32)]),
             ("tlb_mx_grad_workspace", i64, [i32, i64, i64, rows, rows, ptr, i32, ptr, i32]),
             ("tlb_mx_grad", C.c_int, [ptr, i32, i64, i64, rows, rows, ptr, i32, ptr, i32, ptr, i64, ptr])):

@@ -257,6 +257,16 @@ int tlb_mx_matmul(const tlb_mx_rows* a, const tlb_mx_rows* b, void* out, int32_t
     return TLB_OK;
 }
 
+int tlb_mx_linear(const tlb_mx_rows* a, const void* x, int32_t x_dtype, int64_t x_pitch, const tlb_mx_rows* b, const void* w,
+                  int32_t w_dtype, int64_t w_pitch, void* out, int32_t out_dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+    if (int rc = check_product(a, b, out_dtype)) return rc;
+    if (x)
+        if (int rc = tlb_mx_quantize(a, x, x_dtype, x_pitch, stream)) return rc;
+    if (w)
+        if (int rc = tlb_mx_quantize(b, w, w_dtype, w_pitch, stream)) return rc;
+    return tlb_mx_matmul(a, b, out, out_dtype, workspace, workspace_bytes, stream);
+}
+
 int tlb_mx_incomplete(uint32_t* count) {
     if (!count) return fail(TLB_ERR_INVALID_ARG, "count is NULL");
     *count = 0;

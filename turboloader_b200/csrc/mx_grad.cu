@@ -13,7 +13,7 @@
 // The tensor cores cut where they add to an accumulator, about 1e-8 of a sum for every 16 of its terms.  That
 // is below the rounding of a 16-bit result; a result of 32 bits (EXACT) takes the accumulators out every
 // kExactStages stages and adds them in registers, rounding to nearest (12544 x 1000 x 1024, g fp32: 7.4e-6 off
-// without it, EXACTERR with it).
+// without it, 1.6e-7 with it).
 // With few tiles and a long sum, the sum is split; the parts go to a workspace in fp32 and add_kernel adds
 // them in order, so that the result does not depend on which part ends first.
 #include <atomic>
@@ -24,8 +24,9 @@ namespace tlb {
 namespace {
 
 constexpr int kTileM = 128, kDepth = 64;  // rows of a CTA, of the sum a stage
-constexpr int kStageA = kTileM * kDepth * 2, kStageB = 128 * kDepth * 2, kStageBytes = kStageA + kStageB, kStages = 6;
-constexpr int kSmem = 1024 + kStages * kStageBytes + 8 * kStaging;
+constexpr int kStageA = kTileM * kDepth * 2, kBoxB = 64 * kDepth * 2;  // bytes; kBoxB: 64 columns
+constexpr int kRing = 6 * (kStageA + 2 * kBoxB), kMaxStages = kRing / (kStageA + kBoxB);  // 6 stages of 256 columns, 8 of 128
+constexpr int kSmem = 1024 + kRing + 8 * kStaging;
 constexpr int kThreads = 384, kPairs = kSms / 2;
 static_assert(kSmem <= 227 * 1024 - 512, "shared memory");
 constexpr unsigned kTmemColumns = 512;
@@ -69,7 +70,7 @@ struct Item {
 template <typename T, bool EXACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_kernel(const __grid_constant__ GradParams gp) {
     extern __shared__ unsigned char raw[];
-    __shared__ unsigned long long bars[2 * kStages + 4];
+    __shared__ unsigned long long bars[2 * kMaxStages + 4];
     __shared__ unsigned tmem_base;
     __shared__ int gave_up;
     const unsigned smem = (smem_u32(raw) + 1023u) & ~1023u;
@@ -77,9 +78,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
     const unsigned rank = __shfl_sync(0xffffffffu, cluster_rank(), 0);
     const int items = gp.m_tiles * gp.n_tiles * gp.splits, first_item = blockIdx.x / 2, step = gridDim.x / 2;
 
-    const unsigned full = smem_u32(bars), empty = full + 8 * kStages, acc_full = empty + 8 * kStages, acc_empty = acc_full + 16;
+    const unsigned full = smem_u32(bars), empty = full + 8 * kMaxStages, acc_full = empty + 8 * kMaxStages, acc_empty = acc_full + 16;
+    const int b_boxes = gp.tile_n / 128;  // boxes of 64 columns that this CTA's half of B takes
+    const unsigned stage_bytes = kStageA + b_boxes * kBoxB, ring = kRing / stage_bytes;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kStages; ++s) {
+        for (int s = 0; s < kMaxStages; ++s) {
             mbar_init(full + 8 * s, 1);
             mbar_init(empty + 8 * s, 1);
         }
@@ -101,11 +104,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
     const unsigned tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
     volatile int* stop = &gave_up;
     wait_for_previous();
-    const int b_boxes = gp.tile_n / 128;  // boxes of 64 columns that this CTA's half of B takes
 
     if (warp == 0) {
         const bool issue = elect_one();
-        const unsigned full_at = at_leader(full), bytes = kStageA + b_boxes * 8192;
+        const unsigned full_at = at_leader(full), bytes = stage_bytes;
         Ring r;
         unsigned started = 0;
         bool ok = true;
@@ -117,7 +119,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
                 ok = mbar_wait(empty + 8 * r.s, r.parity ^ 1, stop);
                 if (!ok) break;
                 if (issue) {
-                    const unsigned a = smem + r.s * kStageBytes, b = a + kStageA, bar = full_at + 8 * r.s;
+                    const unsigned a = smem + r.s * stage_bytes, b = a + kStageA, bar = full_at + 8 * r.s;
                     if (rank == 0) mbar_arrive_tx(full + 8 * r.s, 2 * bytes);
                     if (gp.transpose) {  // terms are stacked along g's rows, which the sum runs over
                         const int row = term * static_cast<int>(gp.sum) + at * kDepth;
@@ -129,15 +131,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
                     for (int j = 0; j < b_boxes; ++j) tma_load_2d(b + j * 8192, &gp.map_b, n0 + j * 64, at * kDepth, bar);
                 }
                 __syncwarp();
-                r.next(kStages);
+                r.next(ring);
                 ++started;
                 if (++at == gp.term_stages) at = 0, ++term;
             }
         }
         if (*stop && rank == 0) {  // every copy that was started lands before the pair ends
             int none = 0;
-            for (unsigned j = 0; j < kStages && j < started; ++j) {
-                r.back(kStages);
+            for (unsigned j = 0; j < ring && j < started; ++j) {
+                r.back(ring);
                 mbar_wait(full + 8 * r.s, r.parity, &none);
             }
         }
@@ -163,7 +165,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
                     ok = mbar_wait(full + 8 * r.s, r.parity, stop);
                     if (!ok) break;
                     tc_fence_after();
-                    const unsigned a = smem + r.s * kStageBytes, b = a + kStageA;
+                    const unsigned a = smem + r.s * stage_bytes, b = a + kStageA;
                     const unsigned long long da = gp.transpose ? smem_desc(a, 8192, 1024, 2) : smem_desc(a, 16, 1024, 2), db = smem_desc(b, 8192, 1024, 2);
                     if (issue) {
 #pragma unroll
@@ -172,13 +174,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
                         if (kt == to - 1) tc_commit(acc_full + 8 * buf);
                     }
                     __syncwarp();
-                    r.next(kStages);
+                    r.next(ring);
                 }
             }
         }
     } else if (warp >= 4) {
         const int quarter = warp % 4, half = (warp - 4) / 4;
-        const unsigned staging = smem + kStages * kStageBytes + (warp - 4) * kStaging;
+        const unsigned staging = smem + kRing + (warp - 4) * kStaging;
         const float alpha = gp.scaled ? mx_tensor_scale(gp.q) : 1.0f;
         const unsigned acc_empty_at = at_leader(acc_empty);
         unsigned count = 0;
@@ -380,7 +382,7 @@ Shared shared_of(const MxGrad& p) {
     Shared s{};
     s.terms = terms_of(p.g_dtype);
     s.copy_g = s.terms > 1 || p.n % 8 != 0;
-    s.g_pitch = (p.n + 7) / 8 * 8;
+    s.g_pitch = s.copy_g ? (p.n + 63) / 64 * 64 : p.n;  // whole 128-byte lines where g is rewritten anyway
     s.g_bytes = s.copy_g ? round_256(static_cast<size_t>(s.terms) * p.m * s.g_pitch * 2) : 0;
     s.a_bytes = p.grad_b ? round_256(static_cast<size_t>(p.m) * mx_padded(p.a.cols) * 2) : 0;
     s.b_bytes = p.grad_a ? round_256(static_cast<size_t>(p.n) * mx_padded(p.b.cols) * 2) : 0;
@@ -455,13 +457,15 @@ int launch_grad(const GradParams& gp, cudaStream_t st, bool after_operands) {
 // g: its terms, rows of g_pitch elements; values: of the other operand; parts: workspace of a split sum.
 template <typename T>
 int one_grad(const MxGrad& p, const Shared& sh, bool of_b, const void* g, const void* values, void* parts, void* result, bool after_operands, cudaStream_t st) {
-    GradParams gp = plan(p, sh, of_b);
-    if (gp.rows == 0) return 0;
-    if (gp.sum == 0) {
-        zero_kernel<T><<<blocks(gp.rows * gp.cols), 256, 0, st>>>(static_cast<T*>(result), gp.rows * gp.cols);
+    const long long rows = of_b ? p.n : p.m, sum = of_b ? p.m : p.n;
+    if (rows == 0) return 0;
+    if (sum == 0) {
+        const long long total = rows * (of_b ? p.a.cols : p.b.cols);
+        zero_kernel<T><<<blocks(total), 256, 0, st>>>(static_cast<T*>(result), total);
         mx_count_launch();
         return last_error();
     }
+    GradParams gp = plan(p, sh, of_b);
     const unsigned long long g_rows = static_cast<unsigned long long>(sh.terms) * p.m;
     if (int e = mx_encode_map(&gp.map_a, 2, g, p.n, g_rows, sh.g_pitch * 2ull, 64, gp.transpose ? kDepth : kTileM, 1)) return e;
     if (int e = mx_encode_map(&gp.map_b, 2, values, gp.cols, gp.q.rows, mx_padded(gp.cols) * 2ull, 64, kDepth, 1)) return e;

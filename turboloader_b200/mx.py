@@ -6,7 +6,9 @@ written sample by sample, served in shuffled order, and goes through the next mo
 being widened first.  The formats, the layout of the rows and the rules for special values stand in
 ``include/turboloader_b200.h`` ("microscaled rows").  torch allocates memory and names the current stream; every
 computation happens inside the C-ABI library, on the current stream (or ``stream``), without synchronisation, so
-all of it can be captured into CUDA graphs.
+all of it can be captured into CUDA graphs.  With ``stream``, what a call allocates belongs to that stream, and
+ordering it behind the work that makes the inputs (and before what reads the results) is the caller's, as with
+any torch call under ``torch.cuda.stream``.
 
 No counterpart in the reference, whose resident loader keeps uint8 pixels (turboloader/cuda_loader.py:385-535).
 """
@@ -113,9 +115,10 @@ def _on(device, stream):
 
 
 def _rows_struct(codes, scales, rows, cols, fmt, scale):
+    """tlb_mx_rows of two addresses."""
     if isinstance(scale, torch.Tensor):
-        return _capi.MxRows(codes.data_ptr(), scales.data_ptr(), rows, cols, fmt, 1.0, scale.data_ptr())
-    return _capi.MxRows(codes.data_ptr(), scales.data_ptr(), rows, cols, fmt, scale, None)
+        return _capi.MxRows(codes, scales, rows, cols, fmt, 1.0, scale.data_ptr())
+    return _capi.MxRows(codes, scales, rows, cols, fmt, scale, None)
 
 
 def _check_held(codes, scales, rows, cols, fmt):
@@ -164,7 +167,7 @@ class MxTensor:
         return self.codes.device
 
     def _struct(self):
-        return _rows_struct(self.codes, self.scales, self._rows, self.shape[-1], self._fmt, self.scale)
+        return _rows_struct(self.codes.data_ptr(), self.scales.data_ptr(), self._rows, self.shape[-1], self._fmt, self.scale)
 
     def dequantize(self, dtype=torch.float32):
         return mx_dequantize(self, dtype)
@@ -281,19 +284,19 @@ def mx_incomplete() -> int:
     return int(count.value)
 
 
-def _grads(g, qa, qb, a_dtype, b_dtype):
-    """(grad_a, grad_b) of values(a) @ values(b).T for g (m, n); a dtype of None: not wanted."""
+def _grads(g, a, b, cols, a_dtype, b_dtype):
+    """(grad_a, grad_b) of values(a) @ values(b).T for g (m, n); a, b: tlb_mx_rows, needed for the other one's
+    gradient; a dtype of None: not wanted."""
     lib = _capi.load()
     device = g.device
     m, n = g.shape
-    cols = (qa or qb).shape[-1]
     gt = _DTYPES[g.dtype]
     with _on(device, None) as handle:
         ga = None if a_dtype is None else torch.empty((m, cols), dtype=a_dtype, device=device)
         gb = None if b_dtype is None else torch.empty((n, cols), dtype=b_dtype, device=device)
         # an empty tensor has no address; any other one says that its gradient is wanted
-        at = (None if gb is None else qa._struct(), None if ga is None else qb._struct(), None if ga is None else ga.data_ptr() or 16,
-              _DTYPES.get(a_dtype, 0), None if gb is None else gb.data_ptr() or 16, _DTYPES.get(b_dtype, 0))
+        at = (a, b, None if ga is None else ga.data_ptr() or 16, _DTYPES.get(a_dtype, 0), None if gb is None else gb.data_ptr() or 16,
+              _DTYPES.get(b_dtype, 0))
         size = lib.tlb_mx_grad_workspace(gt, m, n, *at)
         ws = _workspace(size, device)
         _capi.check(lib.tlb_mx_grad(g.data_ptr(), gt, m, n, *at, None if ws is None else ws.data_ptr(), size, handle))
@@ -310,35 +313,79 @@ def _spaced(x):
         return x.contiguous()
 
 
+def _align(n):
+    return (n + 255) & ~255
+
+
 class _MxLinear(torch.autograd.Function):
+    """Operands quantised here live in one buffer; `parts` say where, as (saved tensor or tensors, offsets of codes and
+    scales, rows, scale)."""
+
     @staticmethod
     def forward(ctx, x, weight, held_x, held_w, format, scale, weight_scale, dtype):
         fmt = _FORMATS[format]
-        qx = held_x if x is None else _quantize(_spaced(x), format, fmt, scale)
-        qw = held_w if weight is None else _quantize(_spaced(weight), format, fmt, weight_scale)
+        lib = _capi.load()
+        device = (held_x.codes if x is None else x).device
+        cols = (held_x.shape if x is None else x.shape)[-1]
+        cp, sp = _pitches(fmt, cols)
+        at, given, plans = 0, [], []
+        for t, q, s in ((x, held_x, scale), (weight, held_w, weight_scale)):
+            if t is None:
+                given.append((None, 0, 0))
+                plans.append((q, 0, 0, q._rows, q.scale))
+                continue
+            t = _spaced(t)
+            rows, _, pitch = _as_rows(t, "an operand")
+            codes, scales = at, at + _align(rows * cp)
+            at = scales + _align(rows * sp)
+            given.append((t, _DTYPES[t.dtype], pitch))
+            plans.append((None, codes, scales, rows, _check_scale(s, device)))
+        x_shape = held_x.shape if x is None else x.shape
+        dt = _DTYPES[dtype]
+        with _on(device, None) as handle:
+            buf = torch.empty(at, dtype=torch.uint8, device=device) if at else None
+            base = 0 if buf is None else buf.data_ptr()
+            a, b = (q._struct() if q is not None else _rows_struct(base + c, base + s, rows, cols, fmt, ts) for q, c, s, rows, ts in plans)
+            out = torch.empty((*x_shape[:-1], plans[1][3]), dtype=dtype, device=device)
+            size = lib.tlb_mx_matmul_workspace(a, b, dt)
+            ws = _workspace(size, device)
+            (xt, xd, xp), (wt, wd, wp) = given
+            _capi.check(lib.tlb_mx_linear(a, None if xt is None else xt.data_ptr(), xd, xp, b, None if wt is None else wt.data_ptr(), wd, wp,
+                                          out.data_ptr(), dt, None if ws is None else ws.data_ptr(), size, handle))
         needs_x, needs_w = ctx.needs_input_grad[:2]
-        # the gradient of one operand needs the other's codes
-        saved, held = [], []
-        for q, keep in ((qx, needs_w), (qw, needs_x)):
-            held.append((q.shape, q._rows, q.scale) if keep else None)
-            if keep:
-                saved += [q.codes, q.scales]
-        ctx.save_for_backward(*saved)
-        ctx.held, ctx.format, ctx.x_shape = held, format, qx.shape
-        ctx.types = (x.dtype if needs_x else None, weight.dtype if needs_w else None)
-        return _matmul(qx, qw, dtype, _DTYPES[dtype])
+        if needs_x or needs_w:  # the gradient of one operand needs the other's codes
+            keep = [] if buf is None else [buf]
+            for (q, *_), needed in zip(plans, (needs_w, needs_x)):
+                if q is not None and needed:
+                    keep += [q.codes, q.scales]
+            ctx.save_for_backward(*keep)
+            ctx.parts = [(q is not None, c, s, rows, ts) if needed else None for (q, c, s, rows, ts), needed in zip(plans, (needs_w, needs_x))]
+            ctx.one = buf is not None
+            ctx.fmt, ctx.cols, ctx.x_shape = fmt, cols, x_shape
+            ctx.types = (x.dtype if needs_x else None, weight.dtype if needs_w else None)
+        return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         saved = list(ctx.saved_tensors)
-        qx, qw = (None if h is None else MxTensor._made(saved.pop(0), saved.pop(0), h[0], h[1], ctx.format, _FORMATS[ctx.format], h[2])
-                  for h in ctx.held)
+        base = saved.pop(0).data_ptr() if ctx.one else 0
+        ops = []
+        for part in ctx.parts:
+            if part is None:
+                ops.append(None)
+                continue
+            held, c, s, rows, ts = part
+            if held:
+                c, s = saved.pop(0).data_ptr(), saved.pop(0).data_ptr()
+            else:
+                c, s = base + c, base + s
+            ops.append(_rows_struct(c, s, rows, ctx.cols, ctx.fmt, ts))
         if g.dim() != 2 or not g.is_contiguous():
             g = g.reshape(-1, g.shape[-1]).contiguous()
         if g.data_ptr() % 16:
             g = g.clone()
-        gx, gw = _grads(g, qx, qw, *ctx.types)
+        gx, gw = _grads(g, *ops, ctx.cols, *ctx.types)
         return None if gx is None else gx.view(ctx.x_shape), gw, None, None, None, None, None, None
 
 
@@ -415,7 +462,7 @@ class MxCache:
         return 0 if self.status is None else int(self.status.item())
 
     def _struct(self):
-        rows = _rows_struct(self.codes, self.scales, self.slots * self.tokens, self.cols, self._fmt, self.scale)
+        rows = _rows_struct(self.codes.data_ptr(), self.scales.data_ptr(), self.slots * self.tokens, self.cols, self._fmt, self.scale)
         return _capi.MxCache(rows, self.tokens, None if self.lengths is None else self.lengths.data_ptr(),
                              None if self._owner is None else self._owner.data_ptr(),
                              None if self.status is None else self.status.data_ptr())
