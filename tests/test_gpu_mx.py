@@ -487,10 +487,10 @@ def test_captured_without_a_call_before():
 
 def test_offsets_beyond_32_bits():
     """A cache whose codes pass 4 GiB, and a result of more than 2^31 values: their far ends."""
-    slots, tokens, cols = 4100, 256, 4096 + 32
+    slots, tokens, cols = 8200, 256, 4096 + 32
     cache = tb.MxCache(torch.empty(slots, tokens, 2112, dtype=torch.uint8, device="cuda"), torch.empty(slots, tokens, 132, dtype=torch.uint8, device="cuda"),
                        cols, "mxfp4")
-    assert cache.codes.numel() == slots * tokens * 2112 > 2 ** 31
+    assert cache.codes.numel() == slots * tokens * 2112 > 2 ** 32
     x = torch.randn(2, tokens, cols, device="cuda")
     index = torch.tensor([slots - 1, 0], device="cuda")
     cache.write(index, x)
