@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import math
 
 import torch
 
@@ -81,37 +82,23 @@ def _check_scale(scale, device):
     return scale
 
 
+def _away(device, stream):
+    """Whether a call for tensors of ``device`` has to change the current device or stream first."""
+    return stream is not None or torch.cuda.current_device() != device.index
+
+
 @contextlib.contextmanager
-def _elsewhere(device, stream):
-    with torch.cuda.device(device):
-        if stream is None:
-            yield torch.cuda.current_stream(device).cuda_stream
-        else:
-            with torch.cuda.stream(stream):  # outputs and workspaces belong to the stream that uses them
-                yield stream.cuda_stream
-
-
-class _Here:
-    """The usual case of ``_on``: the tensors' device is the current one, and no stream is named."""
-    __slots__ = ("handle",)
-
-    def __init__(self, handle):
-        self.handle = handle
-
-    def __enter__(self):
-        return self.handle
-
-    def __exit__(self, *exc):
-        return False
-
-
-def _on(device, stream):
-    """Context in which the library is called for tensors of ``device``: gives the raw stream."""
-    if stream is None and torch.cuda.current_device() == device.index:
-        return _Here(_raw_stream(device.index))
+def _there(device, stream):
+    """Makes ``device``, and ``stream`` where one is named, the current ones: what a call allocates then belongs to the
+    stream that uses it."""
     if stream is not None and stream.device != device:
         raise ValueError(f"stream is on {stream.device}, the tensors on {device}")
-    return _elsewhere(device, stream)
+    with torch.cuda.device(device):
+        if stream is None:
+            yield
+        else:
+            with torch.cuda.stream(stream):
+                yield
 
 
 def _rows_struct(codes, scales, rows, cols, fmt, scale):
@@ -126,11 +113,11 @@ def _check_held(codes, scales, rows, cols, fmt):
     cp, sp = _pitches(fmt, cols)
     for t, pitch, what in ((codes, cp, "codes"), (scales, sp, "scales")):
         _cuda(t, what)
-        if t.dtype != torch.uint8 or not t.is_contiguous() or t.dim() < 1 or t.shape[-1] != pitch:
+        if t.dtype is not torch.uint8 or not t.is_contiguous() or t.dim() < 1 or t.shape[-1] != pitch:
             raise ValueError(f"{what} must be a contiguous uint8 tensor with rows of {pitch} bytes")
         if t.numel() != rows * pitch:
             raise ValueError(f"{what} must hold {rows} rows, got {t.numel() // pitch}")
-    if codes.device != scales.device:
+    if codes.get_device() != scales.get_device():
         raise ValueError(f"codes are on {codes.device}, scales on {scales.device}")
     if codes.data_ptr() % 16 or scales.data_ptr() % 4:
         raise ValueError("codes must be 16-byte and scales 4-byte aligned")
@@ -141,33 +128,60 @@ class MxTensor:
     says) standing for values of ``shape`` (the last dimension is the rows' length), times ``scale`` -- a float,
     or one float32 value on the device.  Holds the tensors it is given, without a copy."""
 
-    __slots__ = ("codes", "scales", "shape", "format", "scale", "_fmt", "_rows")
+    __slots__ = ("shape", "format", "scale", "device", "_codes", "_scales", "_buf", "_lead", "_fmt", "_rows")
 
     def __init__(self, codes, scales, shape, format, *, scale=1.0):
-        self._fmt = _format_id(format)
-        shape = tuple(int(s) for s in shape)
+        self._fmt = fmt = _format_id(format)
+        self.shape = shape = tuple(shape)
         if not shape:
             raise ValueError("an MxTensor has at least one dimension")
-        self._rows = 1
-        for s in shape[:-1]:
-            self._rows *= s
-        _check_held(codes, scales, self._rows, shape[-1], self._fmt)
-        self.codes, self.scales, self.shape, self.format = codes, scales, shape, format
-        self.scale = 1.0 if scale == 1.0 and not isinstance(scale, torch.Tensor) else _check_scale(scale, codes.device)
+        self._rows = rows = math.prod(shape[:-1])
+        _check_held(codes, scales, rows, shape[-1], fmt)
+        self._codes, self._scales, self.format, self.device, self._buf = codes, scales, format, codes.device, None
+        self.scale = _check_scale(scale, self.device)
 
     @classmethod
-    def _made(cls, codes, scales, shape, rows, format, fmt, scale):
-        """Of tensors that this module made."""
+    def _empty(cls, shape, lead, format, fmt, scale, device):
+        """Room for rows of ``shape``, codes and then scales in one buffer; their tensors, with leading dimensions
+        ``lead``, are made when they are asked for."""
         self = object.__new__(cls)
-        self.codes, self.scales, self.shape, self.format, self.scale, self._fmt, self._rows = codes, scales, shape, format, scale, fmt, rows
+        rows = math.prod(lead)
+        cp, sp = _pitches(fmt, shape[-1])
+        self._buf = torch.empty(rows * (cp + sp), dtype=torch.uint8, device=device)
+        self._codes = self._scales = None
+        self.shape, self._lead, self._rows, self.format, self._fmt, self.scale, self.device = shape, lead, rows, format, fmt, scale, device
         return self
 
+    def _views(self):
+        cp, sp = _pitches(self._fmt, self.shape[-1])
+        at = self._rows * cp
+        self._codes, self._scales = self._buf[:at].view(*self._lead, cp), self._buf[at:].view(*self._lead, sp)
+
     @property
-    def device(self):
-        return self.codes.device
+    def codes(self):
+        if self._codes is None:
+            self._views()
+        return self._codes
+
+    @property
+    def scales(self):
+        if self._scales is None:
+            self._views()
+        return self._scales
+
+    def _at(self):
+        """Addresses of codes and scales."""
+        if self._buf is not None:
+            base = self._buf.data_ptr()
+            return base, base + self._rows * _pitches(self._fmt, self.shape[-1])[0]
+        return self._codes.data_ptr(), self._scales.data_ptr()
+
+    def _tensors(self):
+        """What keeps the rows alive."""
+        return [self._buf] if self._buf is not None else [self._codes, self._scales]
 
     def _struct(self):
-        return _rows_struct(self.codes.data_ptr(), self.scales.data_ptr(), self._rows, self.shape[-1], self._fmt, self.scale)
+        return _rows_struct(*self._at(), self._rows, self.shape[-1], self._fmt, self.scale)
 
     def dequantize(self, dtype=torch.float32):
         return mx_dequantize(self, dtype)
@@ -204,20 +218,16 @@ def mx_quantize(x, format="nvfp4", *, scale=1.0, stream=None):
     contiguous and the rows equally spaced (a slice of a wider matrix will do).  ``scale``: the tensor scale
     that values are divided by first, a float or one float32 value on the device; a power of two loses
     nothing.  For ``nvfp4``, ``max|x| / 2688`` rounded up to a power of two uses the range of its scales."""
-    return _quantize(x, format, _format_id(format), scale, stream)
-
-
-def _quantize(x, format, fmt, scale, stream=None):
-    rows, cols, pitch = _as_rows(x, "x")
+    fmt = _format_id(format)
+    rows, _, pitch = _as_rows(x, "x")
     dt = _dtype_id(x.dtype, "x")
-    cp, sp = _pitches(fmt, cols)
     device = x.device
     scale = _check_scale(scale, device)
-    with _on(device, stream) as handle:
-        codes = torch.empty((rows, cp), dtype=torch.uint8, device=device)
-        scales = torch.empty((rows, sp), dtype=torch.uint8, device=device)
-        q = MxTensor._made(codes, scales, tuple(x.shape), rows, format, fmt, scale)
-        _capi.check(_capi.load().tlb_mx_quantize(q._struct(), x.data_ptr(), dt, pitch, handle))
+    if _away(device, stream):
+        with _there(device, stream):
+            return mx_quantize(x, format, scale=scale)
+    q = MxTensor._empty(tuple(x.shape), (rows,), format, fmt, scale, device)
+    _capi.check(_capi.load().tlb_mx_quantize(q._struct(), x.data_ptr(), dt, pitch, _raw_stream(device.index)))
     return q
 
 
@@ -235,10 +245,13 @@ def _out(out, shape, dtype, device):
 def mx_dequantize(q, dtype=torch.float32, *, out=None, stream=None):
     """The values that ``q`` stands for: code * block scale * tensor scale in fp32, rounded once to ``dtype``."""
     dt = _dtype_id(dtype, "dtype")
-    with _on(q.device, stream) as handle:
-        out = _out(out, q.shape, dtype, q.device)
-        cache = _capi.MxCache(q._struct(), 1, None, None, None)
-        _capi.check(_capi.load().tlb_mx_read(cache, None, q._rows, out.data_ptr(), dt, None, handle))
+    device = q.device
+    if _away(device, stream):
+        with _there(device, stream):
+            return mx_dequantize(q, dtype, out=out)
+    out = _out(out, q.shape, dtype, device)
+    cache = _capi.MxCache(q._struct(), 1, None, None, None)
+    _capi.check(_capi.load().tlb_mx_read(cache, None, q._rows, out.data_ptr(), dt, None, _raw_stream(device.index)))
     return out
 
 
@@ -261,18 +274,17 @@ def mx_matmul(a, b, dtype=torch.bfloat16, *, out=None, stream=None):
     """``a`` (..., k) times the transpose of ``b`` (n, k), two ``MxTensor`` of one format: (..., n) of ``dtype``.
     The products of the codes enter whole and are summed in fp32; the result is rounded once."""
     _check_pair(a, b)
-    return _matmul(a, b, dtype, _dtype_id(dtype, "dtype"), out, stream)
-
-
-def _matmul(a, b, dtype, dt, out=None, stream=None):
+    dt = _dtype_id(dtype, "dtype")
+    device = a.device
+    if _away(device, stream):
+        with _there(device, stream):
+            return mx_matmul(a, b, dtype, out=out)
     lib = _capi.load()
-    device = a.codes.device
-    with _on(device, stream) as handle:
-        out = _out(out, (*a.shape[:-1], b.shape[0]), dtype, device)
-        sa, sb = a._struct(), b._struct()
-        size = lib.tlb_mx_matmul_workspace(sa, sb, dt)
-        ws = _workspace(size, device)
-        _capi.check(lib.tlb_mx_matmul(sa, sb, out.data_ptr(), dt, None if ws is None else ws.data_ptr(), size, handle))
+    out = _out(out, (*a.shape[:-1], b.shape[0]), dtype, device)
+    sa, sb = a._struct(), b._struct()
+    size = lib.tlb_mx_matmul_workspace(sa, sb, dt)
+    ws = _workspace(size, device)
+    _capi.check(lib.tlb_mx_matmul(sa, sb, out.data_ptr(), dt, None if ws is None else ws.data_ptr(), size, _raw_stream(device.index)))
     return out
 
 
@@ -287,19 +299,21 @@ def mx_incomplete() -> int:
 def _grads(g, a, b, cols, a_dtype, b_dtype):
     """(grad_a, grad_b) of values(a) @ values(b).T for g (m, n); a, b: tlb_mx_rows, needed for the other one's
     gradient; a dtype of None: not wanted."""
-    lib = _capi.load()
     device = g.device
+    if _away(device, None):
+        with _there(device, None):
+            return _grads(g, a, b, cols, a_dtype, b_dtype)
+    lib = _capi.load()
     m, n = g.shape
     gt = _DTYPES[g.dtype]
-    with _on(device, None) as handle:
-        ga = None if a_dtype is None else torch.empty((m, cols), dtype=a_dtype, device=device)
-        gb = None if b_dtype is None else torch.empty((n, cols), dtype=b_dtype, device=device)
-        # an empty tensor has no address; any other one says that its gradient is wanted
-        at = (a, b, None if ga is None else ga.data_ptr() or 16, _DTYPES.get(a_dtype, 0), None if gb is None else gb.data_ptr() or 16,
-              _DTYPES.get(b_dtype, 0))
-        size = lib.tlb_mx_grad_workspace(gt, m, n, *at)
-        ws = _workspace(size, device)
-        _capi.check(lib.tlb_mx_grad(g.data_ptr(), gt, m, n, *at, None if ws is None else ws.data_ptr(), size, handle))
+    ga = None if a_dtype is None else torch.empty((m, cols), dtype=a_dtype, device=device)
+    gb = None if b_dtype is None else torch.empty((n, cols), dtype=b_dtype, device=device)
+    # an empty tensor has no address; any other one says that its gradient is wanted
+    at = (a, b, None if ga is None else ga.data_ptr() or 16, _DTYPES.get(a_dtype, 0), None if gb is None else gb.data_ptr() or 16,
+          _DTYPES.get(b_dtype, 0))
+    size = lib.tlb_mx_grad_workspace(gt, m, n, *at)
+    ws = _workspace(size, device)
+    _capi.check(lib.tlb_mx_grad(g.data_ptr(), gt, m, n, *at, None if ws is None else ws.data_ptr(), size, _raw_stream(device.index)))
     return ga, gb
 
 
@@ -318,14 +332,14 @@ def _align(n):
 
 
 class _MxLinear(torch.autograd.Function):
-    """Operands quantised here live in one buffer; `parts` say where, as (saved tensor or tensors, offsets of codes and
-    scales, rows, scale)."""
+    """Operands quantised here live in one buffer; `parts` say where, as (0, offsets of codes and scales, rows, scale);
+    of a held operand the first number counts its saved tensors."""
 
     @staticmethod
     def forward(ctx, x, weight, held_x, held_w, format, scale, weight_scale, dtype):
         fmt = _FORMATS[format]
         lib = _capi.load()
-        device = (held_x.codes if x is None else x).device
+        device = (held_x if x is None else x).device
         cols = (held_x.shape if x is None else x.shape)[-1]
         cp, sp = _pitches(fmt, cols)
         at, given, plans = 0, [], []
@@ -342,24 +356,26 @@ class _MxLinear(torch.autograd.Function):
             plans.append((None, codes, scales, rows, _check_scale(s, device)))
         x_shape = held_x.shape if x is None else x.shape
         dt = _DTYPES[dtype]
-        with _on(device, None) as handle:
-            buf = torch.empty(at, dtype=torch.uint8, device=device) if at else None
-            base = 0 if buf is None else buf.data_ptr()
-            a, b = (q._struct() if q is not None else _rows_struct(base + c, base + s, rows, cols, fmt, ts) for q, c, s, rows, ts in plans)
-            out = torch.empty((*x_shape[:-1], plans[1][3]), dtype=dtype, device=device)
-            size = lib.tlb_mx_matmul_workspace(a, b, dt)
-            ws = _workspace(size, device)
-            (xt, xd, xp), (wt, wd, wp) = given
-            _capi.check(lib.tlb_mx_linear(a, None if xt is None else xt.data_ptr(), xd, xp, b, None if wt is None else wt.data_ptr(), wd, wp,
-                                          out.data_ptr(), dt, None if ws is None else ws.data_ptr(), size, handle))
+        buf = torch.empty(at, dtype=torch.uint8, device=device) if at else None
+        base = 0 if buf is None else buf.data_ptr()
+        a, b = (q._struct() if q is not None else _rows_struct(base + c, base + s, rows, cols, fmt, ts) for q, c, s, rows, ts in plans)
+        out = torch.empty((*x_shape[:-1], plans[1][3]), dtype=dtype, device=device)
+        size = lib.tlb_mx_matmul_workspace(a, b, dt)
+        ws = _workspace(size, device)
+        (xt, xd, xp), (wt, wd, wp) = given
+        _capi.check(lib.tlb_mx_linear(a, None if xt is None else xt.data_ptr(), xd, xp, b, None if wt is None else wt.data_ptr(), wd, wp,
+                                      out.data_ptr(), dt, None if ws is None else ws.data_ptr(), size, _raw_stream(device.index)))
         needs_x, needs_w = ctx.needs_input_grad[:2]
         if needs_x or needs_w:  # the gradient of one operand needs the other's codes
-            keep = [] if buf is None else [buf]
-            for (q, *_), needed in zip(plans, (needs_w, needs_x)):
+            keep, parts = [] if buf is None else [buf], []
+            for (q, c, s, rows, ts), needed in zip(plans, (needs_w, needs_x)):
+                count = 0
                 if q is not None and needed:
-                    keep += [q.codes, q.scales]
+                    keep += q._tensors()
+                    count = len(q._tensors())
+                parts.append((count, c, s, rows, ts) if needed else None)
             ctx.save_for_backward(*keep)
-            ctx.parts = [(q is not None, c, s, rows, ts) if needed else None for (q, c, s, rows, ts), needed in zip(plans, (needs_w, needs_x))]
+            ctx.parts = parts
             ctx.one = buf is not None
             ctx.fmt, ctx.cols, ctx.x_shape = fmt, cols, x_shape
             ctx.types = (x.dtype if needs_x else None, weight.dtype if needs_w else None)
@@ -375,11 +391,12 @@ class _MxLinear(torch.autograd.Function):
             if part is None:
                 ops.append(None)
                 continue
-            held, c, s, rows, ts = part
-            if held:
-                c, s = saved.pop(0).data_ptr(), saved.pop(0).data_ptr()
-            else:
+            count, c, s, rows, ts = part
+            if count == 0:
                 c, s = base + c, base + s
+            else:  # a held operand: one buffer, or its codes and its scales
+                c = saved.pop(0).data_ptr()
+                s = saved.pop(0).data_ptr() if count == 2 else c + rows * _pitches(ctx.fmt, ctx.cols)[0]
             ops.append(_rows_struct(c, s, rows, ctx.cols, ctx.fmt, ts))
         if g.dim() != 2 or not g.is_contiguous():
             g = g.reshape(-1, g.shape[-1]).contiguous()
@@ -415,6 +432,9 @@ def mx_linear(x, weight, format="nvfp4", *, scale=1.0, weight_scale=1.0, dtype=N
     if dtype is None:
         dtype = weight.dtype if held_w is None else x.dtype if held_x is None else torch.bfloat16
     _dtype_id(dtype, "dtype")
+    if _away(x.device, None):
+        with _there(x.device, None):
+            return mx_linear(x, weight, format, scale=scale, weight_scale=weight_scale, dtype=dtype)
     return _MxLinear.apply(None if held_x is not None else x, None if held_w is not None else weight, held_x, held_w,
                            format, scale, weight_scale, dtype)
 
@@ -436,7 +456,7 @@ class MxCache:
         if self.tokens < 1:
             raise ValueError("a cache needs at least one row a sample")
         _check_held(codes, scales, self.slots * self.tokens, self.cols, self._fmt)
-        self.codes, self.scales = codes, scales
+        self.codes, self.scales, self.device = codes, scales, codes.device
         self.lengths = None if lengths is None else _table(lengths, torch.int32, self.slots, codes.device, "lengths")
         self.scale = _check_scale(scale, codes.device)
         self.status = None if status is None else _table(status, torch.int32, 1, codes.device, "status")
@@ -452,10 +472,6 @@ class MxCache:
                    torch.zeros((int(slots), int(tokens), sp), dtype=torch.uint8, device=device), cols, format,
                    lengths=torch.zeros(int(slots), dtype=torch.int32, device=device) if ragged else None, scale=scale,
                    status=torch.zeros(1, dtype=torch.int32, device=device))
-
-    @property
-    def device(self):
-        return self.codes.device
 
     def device_status(self) -> int:
         """Status bits the kernels OR-ed so far (synchronises); 0 when every index and length was valid."""
@@ -493,14 +509,15 @@ class MxCache:
             raise ValueError("the values of a row of x must be contiguous")
         if (self.tokens > 1 and x.stride(1) < self.cols) or (n > 1 and x.stride(0) < self.cols):
             raise ValueError("the rows of x overlap")
-        with _on(device, stream) as handle:
-            if self._owner is None and n > _capi.MX_SCAN_SAMPLES:
-                if torch.cuda.is_current_stream_capturing():
-                    raise RuntimeError(f"write more than {_capi.MX_SCAN_SAMPLES} samples once before the capture: the first such call allocates")
-                self._owner = torch.full((self.slots,), -1, dtype=torch.int32, device=device)
-            _capi.check(_capi.load().tlb_mx_write(self._struct(), index.data_ptr(), n, x.data_ptr(), dt,
-                                                  x.stride(1), x.stride(0), None if lengths is None else lengths.data_ptr(),
-                                                  handle))
+        if _away(device, stream):
+            with _there(device, stream):
+                return self.write(index, x, lengths=lengths)
+        if self._owner is None and n > _capi.MX_SCAN_SAMPLES:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"write more than {_capi.MX_SCAN_SAMPLES} samples once before the capture: the first such call allocates")
+            self._owner = torch.full((self.slots,), -1, dtype=torch.int32, device=device)
+        _capi.check(_capi.load().tlb_mx_write(self._struct(), index.data_ptr(), n, x.data_ptr(), dt, x.stride(1), x.stride(0),
+                                              None if lengths is None else lengths.data_ptr(), _raw_stream(device.index)))
 
     def _picked(self, index):
         if index is None:
@@ -515,11 +532,13 @@ class MxCache:
         n, at = self._picked(index)
         dt = _dtype_id(dtype, "dtype")
         device = self.device
-        with _on(device, stream) as handle:
-            out = _out(out, (n, self.tokens, self.cols), dtype, device)
-            lengths = None if self.lengths is None else torch.empty(n, dtype=torch.int32, device=device)
-            _capi.check(_capi.load().tlb_mx_read(self._struct(), at, n, out.data_ptr(), dt,
-                                                 None if lengths is None else lengths.data_ptr(), handle))
+        if _away(device, stream):
+            with _there(device, stream):
+                return self.read(index, dtype, out=out)
+        out = _out(out, (n, self.tokens, self.cols), dtype, device)
+        lengths = None if self.lengths is None else torch.empty(n, dtype=torch.int32, device=device)
+        _capi.check(_capi.load().tlb_mx_read(self._struct(), at, n, out.data_ptr(), dt, None if lengths is None else lengths.data_ptr(),
+                                             _raw_stream(device.index)))
         return out if lengths is None else (out, lengths)
 
     def read_mx(self, index=None, *, stream=None):
@@ -527,11 +546,11 @@ class MxCache:
         where ``read`` gives zeros; with ``(…, lengths)`` for a cache that has them."""
         n, at = self._picked(index)
         device = self.device
-        with _on(device, stream) as handle:
-            codes = torch.empty((n, self.tokens, self.codes.shape[2]), dtype=torch.uint8, device=device)
-            scales = torch.empty((n, self.tokens, self.scales.shape[2]), dtype=torch.uint8, device=device)
-            lengths = None if self.lengths is None else torch.empty(n, dtype=torch.int32, device=device)
-            _capi.check(_capi.load().tlb_mx_read_codes(self._struct(), at, n, codes.data_ptr(), scales.data_ptr(),
-                                                       None if lengths is None else lengths.data_ptr(), handle))
-        q = MxTensor._made(codes, scales, (n, self.tokens, self.cols), n * self.tokens, self.format, self._fmt, self.scale)
+        if _away(device, stream):
+            with _there(device, stream):
+                return self.read_mx(index)
+        q = MxTensor._empty((n, self.tokens, self.cols), (n, self.tokens), self.format, self._fmt, self.scale, device)
+        lengths = None if self.lengths is None else torch.empty(n, dtype=torch.int32, device=device)
+        _capi.check(_capi.load().tlb_mx_read_codes(self._struct(), at, n, *q._at(), None if lengths is None else lengths.data_ptr(),
+                                                   _raw_stream(device.index)))
         return q if lengths is None else (q, lengths)
