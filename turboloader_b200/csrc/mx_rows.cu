@@ -26,7 +26,7 @@ constexpr int kMaxRounds = 8, kMaxRowsCta = kMaxRounds * kThreads / 4;  // rows 
 static_assert(TLB_MX_SCAN_SAMPLES <= kThreads, "write_kernel reads the index with one load a thread");
 constexpr int kUnit = 16;  // values a thread reads at a time
 // Values a thread quantises at a time: 32 of 16 bits (a whole block, or two), 16 of 32 bits (of a block of 32 lanes
-// 2i and 2i + 1 hold the halves), so that either way two times 64 bytes are on their way to each thread.
+// 2i and 2i + 1 hold the halves): 64 bytes either way.
 template <typename T> constexpr int kTake = sizeof(T) == 2 ? 32 : 16;
 
 // t / s, rounded correctly for the s used here: one step of residual correction of t * (1/s) with
@@ -203,10 +203,11 @@ __global__ void release_kernel(const long long* index, long long n, long long sl
     if (s >= 0 && s < slots) owner[s] = -1;
 }
 
-// One CTA quantises `rows_per_cta` consecutive rows of the call, a thread kTake values at a time, the next ones
-// on their way meanwhile.
+// One CTA quantises `rows_per_cta` consecutive rows of the call, a thread kTake values at a time.  The next values
+// are on their way in other warps: five CTAs an SM that load, then encode, need 23.6 us for 50176 x 1024 bf16
+// values (nvfp4; 5.6 TB/s read and written), four that also load ahead in registers 28.5 us.
 template <typename T, int FMT, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads, ALIGNED ? 4 : 1) write_kernel(MxMove p, int rows_per_cta, SmallDiv by_units, SmallDiv by_tokens) {
+__global__ void __launch_bounds__(kThreads, !ALIGNED ? 1 : sizeof(T) == 2 ? 5 : 4) write_kernel(MxMove p, int rows_per_cta, SmallDiv by_units, SmallDiv by_tokens) {
     const unsigned units = by_units.d;
     const unsigned total = static_cast<unsigned>(p.n * p.tokens);
     const unsigned row0 = blockIdx.x * static_cast<unsigned>(rows_per_cta);
@@ -310,13 +311,10 @@ __global__ void __launch_bounds__(kThreads, ALIGNED ? 4 : 1) write_kernel(MxMove
         else if constexpr (FMT == kNvfp4 || take == 32) sp[w.unit] = static_cast<unsigned char>(bytes);
         else if ((w.unit & 1) == 0) sp[w.unit >> 1] = static_cast<unsigned char>(bytes);
     };
-    Work even, odd;  // whole warps stay together: lanes 2i, 2i + 1 share a block
-    fetch(even, threadIdx.x);
-    for (unsigned u0 = threadIdx.x; u0 - threadIdx.x < all; u0 += 2 * kThreads) {
-        fetch(odd, u0 + kThreads);
-        finish(even);
-        fetch(even, u0 + 2 * kThreads);
-        finish(odd);
+    for (unsigned u0 = threadIdx.x; u0 - threadIdx.x < all; u0 += kThreads) {  // whole warps stay together: lanes 2i, 2i + 1 may share a block
+        Work w;
+        fetch(w, u0);
+        finish(w);
     }
 }
 
@@ -518,10 +516,10 @@ int launch_mx_write(const MxMove& p0, void* stream) {
     MxMove p = p0;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int units = mx_padded(p.q.cols) / (p.dtype == kF32 ? kTake<float> : kTake<__half>);
-    // Rounds of units a thread: one is on its way while another is encoded, so more of them keep more bytes moving, and
-    // the look at the index is shared; fewer where they would leave SMs without work.
+    // Rounds of units a thread: more of them share a CTA's start and its look at the index (12544 CTAs of one round
+    // took twice the time of 1568 of eight); fewer where they would leave SMs without work.
     const long long rounds = p.n * p.tokens * units / (static_cast<long long>(kThreads) * kWriteCtas);
-    const int per_cta = static_cast<int>(rounds < 2 ? 2 : rounds > kMaxRounds ? kMaxRounds : rounds) * kThreads;
+    const int per_cta = static_cast<int>(rounds < 1 ? 1 : rounds > kMaxRounds ? kMaxRounds : rounds) * kThreads;
     const int rows_per_cta = units >= per_cta ? 1 : per_cta / units;
     const long long grid = (p.n * p.tokens + rows_per_cta - 1) / rows_per_cta;
     if (grid > 0x7fffffffll) return static_cast<int>(cudaErrorInvalidValue);
