@@ -183,6 +183,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
         const unsigned staging = smem + kRing + (warp - 4) * kStaging;
         const float alpha = gp.scaled ? mx_tensor_scale(gp.q) : 1.0f;
         const unsigned acc_empty_at = at_leader(acc_empty);
+        const unsigned long long policy = store_policy(false);
         unsigned count = 0;
         const unsigned lanes = tmem + (static_cast<unsigned>(quarter * 32) << 16);
         bool ok = true;
@@ -191,7 +192,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
             const long long in_part = static_cast<long long>(2 * item.m + rank) * kTileM + quarter * 32;
             const int n0 = item.n * gp.tile_n;
             const TileOut<T> to{&gp.map_out, static_cast<T*>(gp.out), gp.pitch, item.split * (static_cast<long long>(gp.m_tiles) * 2 * kTileM) + in_part,
-                                gp.splits > 1 ? 32 : static_cast<int>(min(32ll, gp.rows - in_part)), n0, min(gp.tile_n, gp.cols - n0), gp.vec_ok};
+                                gp.splits > 1 ? 32 : static_cast<int>(min(32ll, gp.rows - in_part)), n0, min(gp.tile_n, gp.cols - n0), gp.vec_ok, policy};
             if constexpr (!EXACT) {
                 const unsigned buf = count & 1;
                 ok = mbar_wait(acc_full + 8 * buf, (count >> 1) & 1, stop);

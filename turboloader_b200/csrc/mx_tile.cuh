@@ -29,6 +29,7 @@ struct TileOut {
     int rows;
     int n0, width;           // the tile's first output column, and how many of its columns there are
     int vec_ok;              // rows are multiples of 16 bytes
+    unsigned long long policy;  // of the stores (store_policy)
 };
 
 // A chunk of 128 bytes of a warp's 32 rows, columns c0 to c0 + 128 / sizeof(T) of the tile, from registers: lane l
@@ -58,7 +59,7 @@ __device__ __forceinline__ void write_chunk(const TileOut<T>& to, const float* v
         fence_async_shared();
         __syncwarp();
         if (lane == 0 && to.rows > 0 && c0 < to.width)
-            tma_store_2d(to.map, (to.n0 + c0) * static_cast<int>(sizeof(T)), static_cast<int>(to.m0), staging);
+            tma_store_2d(to.map, (to.n0 + c0) * static_cast<int>(sizeof(T)), static_cast<int>(to.m0), staging, to.policy);
     } else if (to.vec_ok) {  // the tile's last, narrower chunk
         T* out = to.out + (to.m0 + lane) * to.pitch + to.n0 + c0;
         if (lane < to.rows) {
