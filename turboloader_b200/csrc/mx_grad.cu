@@ -246,12 +246,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
 }
 
 // ---- operands --------------------------------------------------------------------------------------------------
-// Values without the tensor's scale, bf16, rows of `pitch` elements (a multiple of 128); 8 values a thread.
+// Values without the tensor's scale, bf16, rows of `pitch` elements (a multiple of 128); 16 values a thread.
 struct Widen {
     MxRows q;
     __nv_bfloat16* out;
     int pitch;
-    long long units;  // of 8 values
+    long long units;  // of 16 values
 };
 // g as `terms` matrices of bf16, rows of `pitch` elements: each term takes the 8 leading bits of what is left; 8
 // values a thread.
@@ -268,23 +268,29 @@ __device__ __forceinline__ long long quick_div(long long n, int d) {
 
 template <int FMT>
 __device__ __forceinline__ void widen(const Widen& w, long long u) {
-    const int per_row = w.pitch / 8;
+    const int per_row = w.pitch / 16;
     const long long row = quick_div(u, per_row);
     const int unit = static_cast<int>(u - row * per_row);
     const unsigned char* cp = w.q.codes + row * mx_code_pitch(FMT, w.q.cols);
-    const float s = scale_value<FMT>(w.q.scales[row * mx_scale_pitch(FMT, w.q.cols) + unit * 8 / mx_block(FMT)]);
-    float v[8];
+    const float s = scale_value<FMT>(__ldg(w.q.scales + row * mx_scale_pitch(FMT, w.q.cols) + unit / (mx_block(FMT) / 16)));
+    float v[16];
     if (FMT == kMxfp8) {
-        const uint2 c = __ldg(reinterpret_cast<const uint2*>(cp) + unit);
+        const uint4 c = __ldg(reinterpret_cast<const uint4*>(cp) + unit);
         e4m3_values(c.x, v);
         e4m3_values(c.y, v + 4);
+        e4m3_values(c.z, v + 8);
+        e4m3_values(c.w, v + 12);
     } else {
-        e2m1_values(__ldg(reinterpret_cast<const unsigned*>(cp) + unit), v);
+        const uint2 c = __ldg(reinterpret_cast<const uint2*>(cp) + unit);
+        e2m1_values(c.x, v);
+        e2m1_values(c.y, v + 8);
     }
-    __nv_bfloat162 o[4];
+    __nv_bfloat162 o[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = __floats2bfloat162_rn(__fmul_rn(v[2 * i], s), __fmul_rn(v[2 * i + 1], s));
-    *reinterpret_cast<uint4*>(w.out + row * w.pitch + unit * 8) = *reinterpret_cast<const uint4*>(o);
+    for (int i = 0; i < 8; ++i) o[i] = __floats2bfloat162_rn(__fmul_rn(v[2 * i], s), __fmul_rn(v[2 * i + 1], s));
+    uint4* out = reinterpret_cast<uint4*>(w.out + row * w.pitch) + unit * 2;
+    out[0] = reinterpret_cast<const uint4*>(o)[0];
+    out[1] = reinterpret_cast<const uint4*>(o)[1];
 }
 
 __device__ __forceinline__ void split(const Split& p, long long u) {
@@ -523,8 +529,8 @@ int launch_mx_grad(const MxGrad& p, void* stream) {
     unsigned char *a_at = ws + sh.g_bytes, *b_at = a_at + sh.a_bytes, *parts = b_at + sh.b_bytes;
     const bool any = p.m > 0 && p.n > 0;
     if (any) {
-        const Widen a{p.a, reinterpret_cast<__nv_bfloat16*>(a_at), mx_padded(p.a.cols), sh.a_bytes ? p.m * (mx_padded(p.a.cols) / 8) : 0};
-        const Widen b{p.b, reinterpret_cast<__nv_bfloat16*>(b_at), mx_padded(p.b.cols), sh.b_bytes ? static_cast<long long>(p.n) * (mx_padded(p.b.cols) / 8) : 0};
+        const Widen a{p.a, reinterpret_cast<__nv_bfloat16*>(a_at), mx_padded(p.a.cols), sh.a_bytes ? p.m * (mx_padded(p.a.cols) / 16) : 0};
+        const Widen b{p.b, reinterpret_cast<__nv_bfloat16*>(b_at), mx_padded(p.b.cols), sh.b_bytes ? static_cast<long long>(p.n) * (mx_padded(p.b.cols) / 16) : 0};
         const Split g{p.g, p.g_dtype, sh.terms, p.n, sh.g_pitch, p.m, sh.copy_g ? p.m * (sh.g_pitch / 8) : 0, reinterpret_cast<__nv_bfloat16*>(ws)};
         const unsigned n = blocks(a.units + b.units + g.units);
         const int format = p.grad_b ? p.a.format : p.b.format;

@@ -116,6 +116,7 @@ __device__ __forceinline__ void arrange(const Arrange& a, long long t) {
     const int group = static_cast<int>(tile_group % a.groups);
     const long long tile = tile_group / a.groups;
     const int pitch = mx_scale_pitch(a.q.format, a.q.cols) / 4;
+    const bool whole = pitch % 4 == 0 && (reinterpret_cast<unsigned long long>(a.q.scales) & 15u) == 0;  // rows of 16-byte pieces
     unsigned w[4][4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
@@ -123,8 +124,13 @@ __device__ __forceinline__ void arrange(const Arrange& a, long long t) {
         const long long row = tile * a.tile_rows + in_tile;
         const bool there = in_tile < a.tile_rows && row < a.q.rows;
         const unsigned* s = reinterpret_cast<const unsigned*>(a.q.scales) + (there ? row : 0) * pitch;
+        if (whole) {
+            const uint4 v = there && quad * 4 < pitch ? __ldg(reinterpret_cast<const uint4*>(s) + quad) : make_uint4(0u, 0u, 0u, 0u);
+            w[0][c] = v.x, w[1][c] = v.y, w[2][c] = v.z, w[3][c] = v.w;
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i][c] = there && quad * 4 + i < pitch ? __ldg(s + quad * 4 + i) : 0u;
+            for (int i = 0; i < 4; ++i) w[i][c] = there && quad * 4 + i < pitch ? __ldg(s + quad * 4 + i) : 0u;
+        }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -132,9 +138,10 @@ __device__ __forceinline__ void arrange(const Arrange& a, long long t) {
             reinterpret_cast<uint4*>(a.out)[((tile * a.words + quad * 4 + i) * a.groups + group) * 32 + l] = make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]);
 }
 
-__global__ void __launch_bounds__(256) arrange_kernel(Arrange a, Arrange b) {
+constexpr int kArrangeThreads = 128;
+__global__ void __launch_bounds__(kArrangeThreads) arrange_kernel(Arrange a, Arrange b) {
     let_next_start();
-    const long long t = blockIdx.x * 256ll + threadIdx.x;
+    const long long t = blockIdx.x * static_cast<long long>(kArrangeThreads) + threadIdx.x;
     if (t < a.threads) arrange(a, t);
     else if (t - a.threads < b.threads) arrange(b, t - a.threads);
 }
@@ -463,7 +470,7 @@ int launch_mx_matmul(const MxProduct& p, void* stream) {
     const int quads = (a.words + 3) / 4;
     a.threads = 2 * tp.m_tiles * 32 * quads;
     b.threads = static_cast<long long>(tp.n_tiles) * tp.groups_n * 32 * quads;
-    arrange_kernel<<<static_cast<unsigned>((a.threads + b.threads + 255) / 256), 256, 0, st>>>(a, b);
+    arrange_kernel<<<static_cast<unsigned>((a.threads + b.threads + kArrangeThreads - 1) / kArrangeThreads), kArrangeThreads, 0, st>>>(a, b);
     mx_count_launch();
     if (int e = last_error()) return e;
     if (p.out_dtype == kF32) return by_format<float>(tp, st);
