@@ -70,7 +70,7 @@ struct Item {
 template <typename T, bool EXACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_kernel(const __grid_constant__ GradParams gp) {
     extern __shared__ unsigned char raw[];
-    __shared__ unsigned long long bars[2 * kMaxStages + 4];
+    __shared__ unsigned long long bars[2 * kMaxStages + 5];
     __shared__ unsigned tmem_base;
     __shared__ int gave_up;
     const unsigned smem = (smem_u32(raw) + 1023u) & ~1023u;
@@ -78,7 +78,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
     const unsigned rank = __shfl_sync(0xffffffffu, cluster_rank(), 0);
     const int items = gp.m_tiles * gp.n_tiles * gp.splits, first_item = blockIdx.x / 2, step = gridDim.x / 2;
 
-    const unsigned full = smem_u32(bars), empty = full + 8 * kMaxStages, acc_full = empty + 8 * kMaxStages, acc_empty = acc_full + 16;
+    const unsigned full = smem_u32(bars), empty = full + 8 * kMaxStages, acc_full = empty + 8 * kMaxStages, acc_empty = acc_full + 16, drained = acc_empty + 16;
     const int b_boxes = gp.tile_n / 128;  // boxes of 64 columns that this CTA's half of B takes
     const unsigned stage_bytes = kStageA + b_boxes * kBoxB, ring = kRing / stage_bytes;
     if (threadIdx.x == 0) {
@@ -90,6 +90,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
             mbar_init(acc_full + 8 * b, 1);
             mbar_init(acc_empty + 8 * b, 16);
         }
+        mbar_init(drained, 1);
         gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         tma_prefetch_map(&gp.map_a);
@@ -177,6 +178,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
                     r.next(ring);
                 }
             }
+        }
+        if (*stop) {  // the instructions issued so far are done before TMEM is freed
+            int none = 0;
+            if (issue) tc_commit(drained);
+            __syncwarp();
+            mbar_wait(drained, 0, &none);
         }
     } else if (warp >= 4) {
         const int quarter = warp % 4, half = (warp - 4) / 4;

@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(kArrangeThreads) arrange_kernel(Arrange a, Arr
 template <typename T, int FMT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ TileParams tp) {
     extern __shared__ unsigned char raw[];
-    __shared__ unsigned long long bars[2 * kStagesB + 4 + 2 * kSlots];
+    __shared__ unsigned long long bars[2 * kStagesB + 4 + 2 * kSlots + 1];
     __shared__ unsigned tmem_base;
     __shared__ int gave_up;
     const unsigned smem = (smem_u32(raw) + 1023u) & ~1023u;
@@ -164,7 +164,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
     const unsigned b_base = smem + (tp.resident ? kSlots * kSlotBytes : kCodesA + kScaleA), b_step = tp.resident ? kStageBBytes : kStageBytes;
 
     const unsigned full = smem_u32(bars), empty = full + 8 * kStagesB, acc_full = empty + 8 * kStagesB, acc_empty = acc_full + 16;
-    const unsigned a_full = acc_empty + 16, a_empty = a_full + 8 * kSlots;
+    const unsigned a_full = acc_empty + 16, a_empty = a_full + 8 * kSlots, drained = a_empty + 8 * kSlots;
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStagesB; ++s) {
             mbar_init(full + 8 * s, 1);
@@ -178,6 +178,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
             mbar_init(a_full + 8 * s, 1);
             mbar_init(a_empty + 8 * s, 1);
         }
+        mbar_init(drained, 1);
         gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         tma_prefetch_map(&tp.map_a);
@@ -305,6 +306,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
                 __syncwarp();
                 r.next(ring);
             }
+        }
+        if (*stop) {  // the instructions issued so far are done before TMEM is freed
+            int none = 0;
+            if (issue) tc_commit(drained);
+            __syncwarp();
+            mbar_wait(drained, 0, &none);
         }
     } else if (warp >= 4) {
         const int quarter = warp % 4, half = (warp - 4) / 4;

@@ -440,32 +440,41 @@ __global__ void __launch_bounds__(kThreads) read_kernel(MxMove p, SmallDiv by_un
     }
 }
 
-// Rows as they are held: codes and scales into packed buffers, zeros behind a sample's length.
-__global__ void __launch_bounds__(kThreads) read_codes_kernel(MxMove p) {
-    const int cw = mx_code_pitch(p.q.format, p.q.cols) / 16, sw = mx_scale_pitch(p.q.format, p.q.cols) / 4;
-    const int words = cw + sw;
-    const long long total = p.n * p.tokens * words;
-    for (long long u = blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x; u < total;
-         u += gridDim.x * static_cast<long long>(kThreads)) {
-        const long long row = u / words;
-        const int w = static_cast<int>(u - row * words);
-        const long long i = row / p.tokens;
-        const int token = static_cast<int>(row - i * p.tokens);
+// Rows as they are held: codes and scales into packed buffers, zeros behind a sample's length.  A row is `cw` words of
+// 16 bytes of codes, then words of 4 bytes of scales; a thread has kReadUnits words on their way.
+__global__ void __launch_bounds__(kThreads) read_codes_kernel(MxMove p, SmallDiv by_words, SmallDiv by_tokens, unsigned cw) {
+    const unsigned words = by_words.d, sw = words - cw;
+    const unsigned long long total = static_cast<unsigned long long>(p.n) * p.tokens * words, u0 = blockIdx.x * static_cast<unsigned long long>(kReadUnits * kThreads);
+    const unsigned row0 = (u0 >> 32) == 0 ? static_cast<unsigned>(u0) / words : static_cast<unsigned>(u0 / words), off0 = static_cast<unsigned>(u0 - static_cast<unsigned long long>(row0) * words);
+    const unsigned sample0 = p.tokens == 1 ? row0 : row0 / p.tokens, token0 = row0 - sample0 * p.tokens;
+    const unsigned here = static_cast<unsigned>(min(static_cast<unsigned long long>(kReadUnits * kThreads), total - u0));
+    uint4 v[kReadUnits];
+    unsigned row[kReadUnits], word[kReadUnits];
+#pragma unroll
+    for (int j = 0; j < kReadUnits; ++j) {
+        const unsigned u = j * kThreads + threadIdx.x, r = by_words(off0 + u), over = by_tokens(token0 + r);
+        word[j] = off0 + u - r * words;
+        row[j] = row0 + r;
+        v[j] = make_uint4(0u, 0u, 0u, 0u);
+        if (u >= here) continue;
+        const long long i = sample0 + over;
+        const int token = static_cast<int>(token0 + r - over * p.tokens);
         int len;
         const long long s = read_slot(p, i, len);
-        if (w == 0 && token == 0) {
+        if (word[j] == 0 && token == 0) {
             if (s < 0 && p.status) atomicOr(p.status, TLB_DEV_BAD_INDEX);
             if (p.lengths_out) p.lengths_out[i] = len;
         }
-        const bool there = token < len;
-        const long long from = there ? s * p.tokens + token : 0;
-        if (w < cw) {
-            const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-            reinterpret_cast<uint4*>(p.out_codes)[row * cw + w] = there ? reinterpret_cast<const uint4*>(p.q.codes)[from * cw + w] : z;
-        } else {
-            reinterpret_cast<unsigned*>(p.out_scales)[row * sw + w - cw] =
-                there ? reinterpret_cast<const unsigned*>(p.q.scales)[from * sw + w - cw] : 0u;
-        }
+        if (token >= len) continue;
+        const long long from = s * p.tokens + token;
+        if (word[j] < cw) v[j] = __ldg(reinterpret_cast<const uint4*>(p.q.codes) + from * cw + word[j]);
+        else v[j].x = __ldg(reinterpret_cast<const unsigned*>(p.q.scales) + from * sw + (word[j] - cw));
+    }
+#pragma unroll
+    for (int j = 0; j < kReadUnits; ++j) {
+        if (j * kThreads + threadIdx.x >= here) continue;
+        if (word[j] < cw) reinterpret_cast<uint4*>(p.out_codes)[static_cast<long long>(row[j]) * cw + word[j]] = v[j];
+        else reinterpret_cast<unsigned*>(p.out_scales)[static_cast<long long>(row[j]) * sw + (word[j] - cw)] = v[j].x;
     }
 }
 
@@ -500,11 +509,6 @@ int read_by_format(const MxMove& p, cudaStream_t st) {
     if (whole) read_whole_or_not<T, true>(p, static_cast<unsigned>(grid), st);
     else read_whole_or_not<T, false>(p, static_cast<unsigned>(grid), st);
     return 0;
-}
-
-int grid_for(long long threads) {
-    const long long ctas = (threads + kThreads - 1) / kThreads;
-    return static_cast<int>(ctas < 148 * 64 ? ctas : 148 * 64);
 }
 
 }  // namespace
@@ -551,8 +555,10 @@ int launch_mx_read(const MxMove& p, void* stream) {
 
 int launch_mx_read_codes(const MxMove& p, void* stream) {
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int words = mx_code_pitch(p.q.format, p.q.cols) / 16 + mx_scale_pitch(p.q.format, p.q.cols) / 4;
-    read_codes_kernel<<<grid_for(p.n * p.tokens * words), kThreads, 0, st>>>(p);
+    const int cw = mx_code_pitch(p.q.format, p.q.cols) / 16, words = cw + mx_scale_pitch(p.q.format, p.q.cols) / 4;
+    const long long ctas = (p.n * p.tokens * words + kReadUnits * kThreads - 1) / (kReadUnits * kThreads);
+    if (ctas > 0x7fffffffll) return static_cast<int>(cudaErrorInvalidValue);
+    read_codes_kernel<<<static_cast<unsigned>(ctas), kThreads, 0, st>>>(p, SmallDiv(words), SmallDiv(p.tokens), cw);
     mx_count_launch();
     return static_cast<int>(cudaGetLastError());
 }
