@@ -359,7 +359,7 @@ TLB_API void tlb_epoch_destroy(tlb_epoch* e);
  *
  * A block of consecutive values of a row shares one 8-bit scale.  With t = fp32(x / tensor scale) and
  * a = max |t| of the block (roundings to nearest even, saturating):
- *   TLB_MX_NVFP4  16 values: scale s = e4m3(a / 6),                   codes e2m1(t / s)
+ *   TLB_MX_NVFP4  16 values: scale s = e4m3(fp32(a * fp32(1/6))),     codes e2m1(t / s)
  *   TLB_MX_MXFP4  32 values: scale s = 2^max(floor(log2 a) - 2, -127), codes e2m1(t / s)
  *   TLB_MX_MXFP8  32 values: scale s = 2^max(floor(log2 a) - 8, -127), codes e4m3(t / s)
  * An nvfp4 scale that rounds to zero makes its codes zero.  A block that holds an infinity or a NaN

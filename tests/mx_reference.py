@@ -30,7 +30,7 @@ def encode(x, fmt, scale=1.0):
     t = np.where(bad[..., None], 0.0, t)
     a = np.abs(t).max(-1)
     if fmt == "nvfp4":
-        sb = nearest(a / 6, E4M3)
+        sb = nearest((a.astype(np.float32) * np.float32(1 / 6)).astype(np.float64), E4M3)
         s = E4M3[sb]
         sb[bad] = 0x7F
     else:

@@ -82,6 +82,25 @@ def test_quantize_of_slices_scales_on_the_device_and_many_dimensions():
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [1, 7, 16, 17, 25, 31, 32, 33, 48, 63, 70, 100, 315])
+def test_quantize_rows_that_end_anywhere_in_aligned_and_odd_matrices(fmt, dtype, cols):
+    """Rows at multiples of 32 bytes, and at every other distance and start, cut off at any column."""
+    for pitch, start in ((320, 0), (328, 0), (321, 0), (336, 3), (352, 16)):
+        wide = _values(37, pitch, dtype, cols + pitch)
+        x = wide[:, start:start + cols]
+        q = tb.mx_quantize(wide.cuda()[:, start:start + cols], fmt)
+        codes, scales = encode(_np(x), fmt)
+        _same(q.codes.cpu().numpy(), codes)
+        _same(q.scales.cpu().numpy(), scales)
+        cache = tb.MxCache.empty(20, 2, cols, fmt)
+        index = torch.arange(18, device="cuda")
+        cache.write(index, wide[:36].cuda().view(18, 2, pitch)[:, :, start:start + cols])
+        _same(cache.codes[:18].reshape(36, -1).cpu().numpy(), codes[:36])
+        _same(cache.scales[:18].reshape(36, -1).cpu().numpy(), scales[:36])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 def test_every_float16_value_and_every_code(fmt):
     """All finite float16 values, one block each beside a fixed largest value, and every byte a row can hold."""
     bits = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(torch.float16)

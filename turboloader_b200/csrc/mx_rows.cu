@@ -3,10 +3,10 @@
 //
 // Arithmetic of a block (16 values for nvfp4, 32 for mxfp4 / mxfp8) with t = fp32(x / tensor scale),
 // a = max |t|:
-//   nvfp4  s = e4m3(a / 6),                       code = e2m1(t / s)
+//   nvfp4  s = e4m3(fp32(a * fp32(1/6))),         code = e2m1(t / s)
 //   mxfp4  s = 2^max(floor(log2 a) - 2, -127),    code = e2m1(t / s)
 //   mxfp8  s = 2^max(floor(log2 a) - 8, -127),    code = e4m3(t / s)
-// all roundings to nearest even, saturating.  Every code is the one that exact arithmetic on t gives:
+// all roundings to nearest even, saturating.  Given t and s, every code is the one that exact arithmetic gives:
 // powers of two scale exactly, and the nvfp4 quotients are rounded correctly (a quotient of t by the
 // 4-bit significand of s that is not itself a rounding border of e2m1 differs from the border by more
 // than half a step of fp32, so the rounded quotient never lands on the wrong side of it).
@@ -64,7 +64,7 @@ __device__ __forceinline__ unsigned encode(float t[N], unsigned c[], bool few_bi
         unsigned byte;
         if (FMT == kNvfp4) {
             unsigned short b2;
-            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(b2) : "f"(0.0f), "f"(quotient(__uint_as_float(a), 6.0f, 1.0f / 6.0f)));
+            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(b2) : "f"(0.0f), "f"(__fmul_rn(__uint_as_float(a), 1.0f / 6.0f)));
             byte = b2 & 0xffu;
             const float inv = inverse[byte];
             if (few_bits) {
@@ -126,7 +126,7 @@ struct Raw {
                         if constexpr (sizeof(T) == 4) {
                             v[i] = i < have ? __ldg(reinterpret_cast<const unsigned*>(p) + 8 * j + i) : 0u;
                         } else {
-                            const unsigned short* h = reinterpret_cast<const unsigned short*>(p) + 2 * i;
+                            const unsigned short* h = reinterpret_cast<const unsigned short*>(p) + 16 * j + 2 * i;
                             v[i] = (2 * i < have ? __ldg(h) : 0u) | (2 * i + 1 < have ? static_cast<unsigned>(__ldg(h + 1)) << 16 : 0u);
                         }
                     }
