@@ -441,6 +441,40 @@ def test_another_stream_gives_the_same_results():
     torch.cuda.synchronize()
 
 
+def test_calls_on_several_streams_at_once():
+    """Products, gradients, writes and reads that overlap in time, each on data of its own."""
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    work, want = [], []
+    for i, fmt in enumerate(("nvfp4", "mxfp4", "mxfp8", "nvfp4")):
+        g = torch.Generator(device="cuda").manual_seed(i)
+        x = torch.randn(700 + 64 * i, 640, generator=g, device="cuda")
+        w = torch.randn(500, 640, generator=g, device="cuda")
+        up = torch.randn(x.shape[0], 500, generator=g, device="cuda")
+        cache = tb.MxCache.empty(400, 2, 640, fmt)
+        index = torch.randperm(400, generator=g, device="cuda")[:300 + i]
+
+        def step(x=x, w=w, up=up, cache=cache, index=index, fmt=fmt):
+            a, b = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+            y = tb.mx_linear(a, b, fmt)
+            ga, gb = torch.autograd.grad(y, [a, b], up)
+            cache.write(index, x[:600].view(300, 2, 640).repeat(2, 1, 1)[:index.shape[0]])
+            return y.detach(), ga, gb, cache.read(index, torch.float32), tb.mx_matmul(tb.mx_quantize(x[:1], fmt), tb.mx_quantize(w, fmt), torch.float32)
+
+        work.append(step)
+        want.append(step())
+    torch.cuda.synchronize()
+    got = [None] * 4
+    for _ in range(5):
+        for i, step in enumerate(work):
+            with torch.cuda.stream(streams[i]):
+                got[i] = step()
+    torch.cuda.synchronize()
+    for have, expected in zip(got, want):
+        for a, b in zip(have, expected):
+            assert torch.equal(a, b)
+    assert tb.mx_incomplete() == 0
+
+
 def test_captured_and_replayed():
     """Two graphs of the whole path with their own workspaces, replayed in turn on changing inputs."""
     n, tokens, cols, out = 12, 3, 160, 200

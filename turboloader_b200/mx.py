@@ -318,67 +318,71 @@ def _grads(g, a, b, cols, a_dtype, b_dtype):
 
 
 def _spaced(x):
-    """``x`` as rows that mx_quantize takes; a copy only where its strides demand one."""
-    x = x.detach()
+    """``x`` as rows that can be quantised, and their number and pitch; a copy only where its strides demand one."""
     try:
-        _as_rows(x, "x")
-        return x
+        rows, _, pitch = _as_rows(x, "x")
     except ValueError:
-        return x.contiguous()
+        x = x.contiguous()
+        rows, _, pitch = _as_rows(x, "x")
+    return x, rows, pitch
 
 
 def _align(n):
     return (n + 255) & ~255
 
 
+def _linear(x, weight, held_x, held_w, fmt, scale, weight_scale, dtype):
+    """The product of mx_linear, and where its operands' rows lie: (out, buffer of those quantised here or None, for each
+    operand (held one or None, offsets of codes and scales in the buffer, rows, scale))."""
+    lib = _capi.load()
+    device = (held_x if x is None else x).device
+    shape = held_x.shape if x is None else x.shape
+    cols = shape[-1]
+    cp, sp = _pitches(fmt, cols)
+    at, given, plans = 0, [], []
+    for t, q, s in ((x, held_x, scale), (weight, held_w, weight_scale)):
+        if t is None:
+            given += None, 0, 0
+            plans.append((q, 0, 0, q._rows, q.scale))
+            continue
+        t, rows, pitch = _spaced(t)
+        codes, scales = at, at + _align(rows * cp)
+        at = scales + _align(rows * sp)
+        given += t, _DTYPES[t.dtype], pitch
+        plans.append((None, codes, scales, rows, _check_scale(s, device)))
+    xt, xd, xp, wt, wd, wp = given
+    dt = _DTYPES[dtype]
+    buf = torch.empty(at, dtype=torch.uint8, device=device) if at else None
+    base = 0 if buf is None else buf.data_ptr()
+    a, b = [q._struct() if q is not None else _rows_struct(base + c, base + s, rows, cols, fmt, ts) for q, c, s, rows, ts in plans]
+    out = torch.empty((*shape[:-1], plans[1][3]), dtype=dtype, device=device)
+    size = lib.tlb_mx_matmul_workspace(a, b, dt)
+    ws = _workspace(size, device)
+    _capi.check(lib.tlb_mx_linear(a, None if xt is None else xt.data_ptr(), xd, xp, b, None if wt is None else wt.data_ptr(), wd, wp,
+                                  out.data_ptr(), dt, None if ws is None else ws.data_ptr(), size, _raw_stream(device.index)))
+    return out, buf, plans
+
+
 class _MxLinear(torch.autograd.Function):
-    """Operands quantised here live in one buffer; `parts` say where, as (0, offsets of codes and scales, rows, scale);
-    of a held operand the first number counts its saved tensors."""
+    """`ctx.parts`: where the operands' rows lie that the backward pass needs, as (0, offsets of codes and scales in the
+    first saved tensor, rows, scale); of a held operand the first number counts its saved tensors."""
 
     @staticmethod
-    def forward(ctx, x, weight, held_x, held_w, format, scale, weight_scale, dtype):
-        fmt = _FORMATS[format]
-        lib = _capi.load()
-        device = (held_x if x is None else x).device
-        cols = (held_x.shape if x is None else x.shape)[-1]
-        cp, sp = _pitches(fmt, cols)
-        at, given, plans = 0, [], []
-        for t, q, s in ((x, held_x, scale), (weight, held_w, weight_scale)):
-            if t is None:
-                given.append((None, 0, 0))
-                plans.append((q, 0, 0, q._rows, q.scale))
-                continue
-            t = _spaced(t)
-            rows, _, pitch = _as_rows(t, "an operand")
-            codes, scales = at, at + _align(rows * cp)
-            at = scales + _align(rows * sp)
-            given.append((t, _DTYPES[t.dtype], pitch))
-            plans.append((None, codes, scales, rows, _check_scale(s, device)))
-        x_shape = held_x.shape if x is None else x.shape
-        dt = _DTYPES[dtype]
-        buf = torch.empty(at, dtype=torch.uint8, device=device) if at else None
-        base = 0 if buf is None else buf.data_ptr()
-        a, b = (q._struct() if q is not None else _rows_struct(base + c, base + s, rows, cols, fmt, ts) for q, c, s, rows, ts in plans)
-        out = torch.empty((*x_shape[:-1], plans[1][3]), dtype=dtype, device=device)
-        size = lib.tlb_mx_matmul_workspace(a, b, dt)
-        ws = _workspace(size, device)
-        (xt, xd, xp), (wt, wd, wp) = given
-        _capi.check(lib.tlb_mx_linear(a, None if xt is None else xt.data_ptr(), xd, xp, b, None if wt is None else wt.data_ptr(), wd, wp,
-                                      out.data_ptr(), dt, None if ws is None else ws.data_ptr(), size, _raw_stream(device.index)))
+    def forward(ctx, x, weight, held_x, held_w, fmt, scale, weight_scale, dtype):
+        out, buf, plans = _linear(x, weight, held_x, held_w, fmt, scale, weight_scale, dtype)
         needs_x, needs_w = ctx.needs_input_grad[:2]
-        if needs_x or needs_w:  # the gradient of one operand needs the other's codes
-            keep, parts = [] if buf is None else [buf], []
-            for (q, c, s, rows, ts), needed in zip(plans, (needs_w, needs_x)):
-                count = 0
-                if q is not None and needed:
-                    keep += q._tensors()
-                    count = len(q._tensors())
-                parts.append((count, c, s, rows, ts) if needed else None)
-            ctx.save_for_backward(*keep)
-            ctx.parts = parts
-            ctx.one = buf is not None
-            ctx.fmt, ctx.cols, ctx.x_shape = fmt, cols, x_shape
-            ctx.types = (x.dtype if needs_x else None, weight.dtype if needs_w else None)
+        keep, parts = [] if buf is None else [buf], []
+        for (q, c, s, rows, ts), needed in zip(plans, (needs_w, needs_x)):  # the gradient of one needs the other's codes
+            count = 0
+            if q is not None and needed:
+                keep += q._tensors()
+                count = len(q._tensors())
+            parts.append((count, c, s, rows, ts) if needed else None)
+        ctx.save_for_backward(*keep)
+        ctx.parts = parts
+        ctx.one = buf is not None
+        ctx.fmt, ctx.x_shape = fmt, held_x.shape if x is None else x.shape
+        ctx.types = (x.dtype if needs_x else None, weight.dtype if needs_w else None)
         return out
 
     @staticmethod
@@ -386,6 +390,7 @@ class _MxLinear(torch.autograd.Function):
     def backward(ctx, g):
         saved = list(ctx.saved_tensors)
         base = saved.pop(0).data_ptr() if ctx.one else 0
+        cols = ctx.x_shape[-1]
         ops = []
         for part in ctx.parts:
             if part is None:
@@ -396,13 +401,13 @@ class _MxLinear(torch.autograd.Function):
                 c, s = base + c, base + s
             else:  # a held operand: one buffer, or its codes and its scales
                 c = saved.pop(0).data_ptr()
-                s = saved.pop(0).data_ptr() if count == 2 else c + rows * _pitches(ctx.fmt, ctx.cols)[0]
-            ops.append(_rows_struct(c, s, rows, ctx.cols, ctx.fmt, ts))
+                s = saved.pop(0).data_ptr() if count == 2 else c + rows * _pitches(ctx.fmt, cols)[0]
+            ops.append(_rows_struct(c, s, rows, cols, ctx.fmt, ts))
         if g.dim() != 2 or not g.is_contiguous():
             g = g.reshape(-1, g.shape[-1]).contiguous()
         if g.data_ptr() % 16:
             g = g.clone()
-        gx, gw = _grads(g, *ops, ctx.cols, *ctx.types)
+        gx, gw = _grads(g, *ops, cols, *ctx.types)
         return None if gx is None else gx.view(ctx.x_shape), gw, None, None, None, None, None, None
 
 
@@ -415,28 +420,31 @@ def mx_linear(x, weight, format="nvfp4", *, scale=1.0, weight_scale=1.0, dtype=N
     ``dweight = g.T @ values(x)``, with every value of g entering whole, sums in fp32, in the operand's own type;
     for the backward pass only the codes are kept.  An ``MxTensor`` must stay unchanged until then.  ``dtype``
     (the result's): by default ``weight``'s, else ``x``'s, else bfloat16."""
-    _format_id(format)
+    fmt = _format_id(format)
     held_x, held_w = (t if isinstance(t, MxTensor) else None for t in (x, weight))
-    for t, what in ((x, "x"), (weight, "weight")):
-        if isinstance(t, MxTensor):
-            if t.format != format:
-                raise ValueError(f"{what} is {t.format}, not {format}")
+    for t, held, what in ((x, held_x, "x"), (weight, held_w, "weight")):
+        if held is not None:
+            if held._fmt != fmt:
+                raise ValueError(f"{what} is {held.format}, not {format}")
         else:
             _dtype_id(_cuda(t, what).dtype, what)
             if t.dim() < 1:
                 raise ValueError(f"{what} must have at least one dimension")
     if len(weight.shape) != 2 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"shapes {tuple(x.shape)} and {tuple(weight.shape)} do not multiply: weight must be (n, {x.shape[-1]})")
-    if x.device != weight.device:
-        raise ValueError(f"x is on {x.device}, weight on {weight.device}")
+    device = x.device
+    if device != weight.device:
+        raise ValueError(f"x is on {device}, weight on {weight.device}")
     if dtype is None:
         dtype = weight.dtype if held_w is None else x.dtype if held_x is None else torch.bfloat16
     _dtype_id(dtype, "dtype")
-    if _away(x.device, None):
-        with _there(x.device, None):
+    if _away(device, None):
+        with _there(device, None):
             return mx_linear(x, weight, format, scale=scale, weight_scale=weight_scale, dtype=dtype)
-    return _MxLinear.apply(None if held_x is not None else x, None if held_w is not None else weight, held_x, held_w,
-                           format, scale, weight_scale, dtype)
+    args = (None if held_x is not None else x, None if held_w is not None else weight, held_x, held_w, fmt, scale, weight_scale, dtype)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:2]):
+        return _MxLinear.apply(*args)
+    return _linear(*args)[0]
 
 
 class MxCache:
