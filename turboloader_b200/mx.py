@@ -233,7 +233,7 @@ def mx_quantize(x, format="nvfp4", *, scale=1.0, stream=None):
 
 def _out(out, shape, dtype, device):
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return torch.empty(*shape, dtype=dtype, device=device)  # sizes one by one parse faster than a tuple
     _cuda(out, "out")
     if out.dtype != dtype or tuple(out.shape) != tuple(shape) or not out.is_contiguous() or out.device != device:
         raise ValueError(f"out must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}")
@@ -306,8 +306,8 @@ def _grads(g, a, b, cols, a_dtype, b_dtype):
     lib = _capi.load()
     m, n = g.shape
     gt = _DTYPES[g.dtype]
-    ga = None if a_dtype is None else torch.empty((m, cols), dtype=a_dtype, device=device)
-    gb = None if b_dtype is None else torch.empty((n, cols), dtype=b_dtype, device=device)
+    ga = None if a_dtype is None else torch.empty(m, cols, dtype=a_dtype, device=device)
+    gb = None if b_dtype is None else torch.empty(n, cols, dtype=b_dtype, device=device)
     # an empty tensor has no address; any other one says that its gradient is wanted
     at = (a, b, None if ga is None else ga.data_ptr() or 16, _DTYPES.get(a_dtype, 0), None if gb is None else gb.data_ptr() or 16,
           _DTYPES.get(b_dtype, 0))
@@ -355,7 +355,7 @@ def _linear(x, weight, held_x, held_w, fmt, scale, weight_scale, dtype):
     buf = torch.empty(at, dtype=torch.uint8, device=device) if at else None
     base = 0 if buf is None else buf.data_ptr()
     a, b = [q._struct() if q is not None else _rows_struct(base + c, base + s, rows, cols, fmt, ts) for q, c, s, rows, ts in plans]
-    out = torch.empty((*shape[:-1], plans[1][3]), dtype=dtype, device=device)
+    out = torch.empty(*shape[:-1], plans[1][3], dtype=dtype, device=device)
     size = lib.tlb_mx_matmul_workspace(a, b, dt)
     ws = _workspace(size, device)
     _capi.check(lib.tlb_mx_linear(a, None if xt is None else xt.data_ptr(), xd, xp, b, None if wt is None else wt.data_ptr(), wd, wp,
