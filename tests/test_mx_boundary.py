@@ -112,6 +112,18 @@ def test_bad_calls_are_refused():
     assert lib.tlb_mx_matmul(C.byref(q), C.byref(_rows(rows=0)), None, 0, None, 0, None) == 0
     r = C.byref(q)  # 8 rows
 
+    def linear(a=r, x=0x5000, xd=0, xp=64, b=r, w=0x5800, wd=0, wp=64, out=0x6000, od=0, ws=None, size=0):
+        return lib.tlb_mx_linear(a, x, xd, xp, b, w, wd, wp, out, od, ws, size, None)
+
+    need = lib.tlb_mx_matmul_workspace(r, r, 0)
+    assert need > 0 and linear() == 1 and b"workspace" in lib.tlb_last_error()
+    ready = dict(ws=0x8000, size=need)
+    assert linear(xd=3, **ready) == linear(wd=4, **ready) == linear(od=3, **ready) == linear(out=None, **ready) == 1
+    assert linear(xp=63, **ready) == linear(wp=10, **ready) == linear(x=0x5002, **ready) == linear(w=0x5801, wd=1, **ready) == 1
+    assert linear(a=None, **ready) == linear(b=C.byref(_rows(cols=65)), **ready) == linear(b=C.byref(_rows(format=2)), **ready) == 1
+    none = C.byref(_rows(rows=0))
+    assert linear(a=none, b=none, out=None) == 0
+
     def grad(g=0x5000, dtype=0, m=8, n=8, a=r, b=r, ga=0x6000, gb=0x7000, da=0, db=0, ws=None, size=0):
         return lib.tlb_mx_grad(g, dtype, m, n, a, b, ga, da, gb, db, ws, size, None)
 

@@ -112,6 +112,43 @@ tlb::MxProduct product_of(const tlb_mx_rows& a, const tlb_mx_rows& b, int out_dt
     return p;
 }
 
+int check_quantize(const tlb_mx_rows* q, const void* x, int x_dtype, int64_t x_pitch) {
+    if (int rc = check_rows(q, "q")) return rc;
+    if (int rc = check_dtype(x_dtype, "x")) return rc;
+    if (q->rows == 0) return TLB_OK;
+    if (!x) return fail(TLB_ERR_INVALID_ARG, "x is NULL");
+    if (q->rows > 1 && x_pitch < q->cols) return fail(TLB_ERR_INVALID_ARG, "x: row pitch %lld is less than %d columns", static_cast<long long>(x_pitch), q->cols);
+    if (misaligned(x, x_dtype == TLB_F32 ? 4 : 2)) return fail(TLB_ERR_INVALID_ARG, "x is not aligned to its type");
+    return TLB_OK;
+}
+
+int quantize(const tlb_mx_rows& q, const void* x, int x_dtype, int64_t x_pitch, void* stream) {
+    tlb::MxMove p{};
+    p.q = rows_of(q);
+    p.slots = p.n = q.rows;
+    p.tokens = 1;
+    p.in = x;
+    p.dtype = x_dtype;
+    p.row_pitch = 0;
+    p.sample_pitch = x_pitch;
+    if (int e = tlb::launch_mx_write(p, stream)) return cuda_fail(e, "mx_quantize");
+    return TLB_OK;
+}
+
+int check_matmul(tlb::MxProduct& p, const tlb_mx_rows* a, const tlb_mx_rows* b, void* out, int out_dtype, void* workspace, int64_t workspace_bytes) {
+    if (int rc = check_product(a, b, out_dtype)) return rc;
+    if (a->rows == 0 || b->rows == 0) return TLB_OK;
+    if (!out) return fail(TLB_ERR_INVALID_ARG, "out is NULL");
+    if (misaligned(out, 16)) return fail(TLB_ERR_INVALID_ARG, "out needs 16-byte alignment");
+    p = product_of(*a, *b, out_dtype);
+    const int64_t need = static_cast<int64_t>(tlb::mx_matmul_workspace(p));
+    if (need > 0 && (!workspace || workspace_bytes < need || misaligned(workspace, 256)))
+        return fail(TLB_ERR_INVALID_ARG, "workspace of %lld bytes (256-byte aligned) is needed", static_cast<long long>(need));
+    p.out = out;
+    p.workspace = workspace;
+    return TLB_OK;
+}
+
 // Fills p but for its pointers to g and the workspace; the results' only say which are wanted.
 int check_grad(tlb::MxGrad& p, int g_dtype, int64_t m, int64_t n, const tlb_mx_rows* a, const tlb_mx_rows* b, const void* grad_a, int32_t grad_a_dtype,
                const void* grad_b, int32_t grad_b_dtype) {
@@ -157,23 +194,10 @@ int64_t tlb_mx_scale_pitch(int32_t format, int32_t cols) {
 }
 
 int tlb_mx_quantize(const tlb_mx_rows* q, const void* x, int32_t x_dtype, int64_t x_pitch, void* stream) {
-    if (int rc = check_rows(q, "q")) return rc;
-    if (int rc = check_dtype(x_dtype, "x")) return rc;
+    if (int rc = check_quantize(q, x, x_dtype, x_pitch)) return rc;
     if (q->rows == 0) return TLB_OK;
-    if (!x) return fail(TLB_ERR_INVALID_ARG, "x is NULL");
-    if (q->rows > 1 && x_pitch < q->cols) return fail(TLB_ERR_INVALID_ARG, "x: row pitch %lld is less than %d columns", static_cast<long long>(x_pitch), q->cols);
-    if (misaligned(x, x_dtype == TLB_F32 ? 4 : 2)) return fail(TLB_ERR_INVALID_ARG, "x is not aligned to its type");
     if (int rc = need_device()) return rc;
-    tlb::MxMove p{};
-    p.q = rows_of(*q);
-    p.slots = p.n = q->rows;
-    p.tokens = 1;
-    p.in = x;
-    p.dtype = x_dtype;
-    p.row_pitch = 0;
-    p.sample_pitch = x_pitch;
-    if (int e = tlb::launch_mx_write(p, stream)) return cuda_fail(e, "mx_quantize");
-    return TLB_OK;
+    return quantize(*q, x, x_dtype, x_pitch, stream);
 }
 
 int tlb_mx_write(const tlb_mx_cache* cache, const int64_t* index, int64_t n, const void* x, int32_t x_dtype,
@@ -242,29 +266,31 @@ int64_t tlb_mx_matmul_workspace(const tlb_mx_rows* a, const tlb_mx_rows* b, int3
 
 int tlb_mx_matmul(const tlb_mx_rows* a, const tlb_mx_rows* b, void* out, int32_t out_dtype, void* workspace,
                   int64_t workspace_bytes, void* stream) {
-    if (int rc = check_product(a, b, out_dtype)) return rc;
+    tlb::MxProduct p{};
+    if (int rc = check_matmul(p, a, b, out, out_dtype, workspace, workspace_bytes)) return rc;
     if (a->rows == 0 || b->rows == 0) return TLB_OK;
-    if (!out) return fail(TLB_ERR_INVALID_ARG, "out is NULL");
-    if (misaligned(out, 16)) return fail(TLB_ERR_INVALID_ARG, "out needs 16-byte alignment");
-    tlb::MxProduct p = product_of(*a, *b, out_dtype);
-    const int64_t need = static_cast<int64_t>(tlb::mx_matmul_workspace(p));
-    if (need > 0 && (!workspace || workspace_bytes < need || misaligned(workspace, 256)))
-        return fail(TLB_ERR_INVALID_ARG, "workspace of %lld bytes (256-byte aligned) is needed", static_cast<long long>(need));
     if (int rc = need_device()) return rc;
-    p.out = out;
-    p.workspace = workspace;
     if (int e = tlb::launch_mx_matmul(p, stream)) return cuda_fail(e, "mx_matmul");
     return TLB_OK;
 }
 
 int tlb_mx_linear(const tlb_mx_rows* a, const void* x, int32_t x_dtype, int64_t x_pitch, const tlb_mx_rows* b, const void* w,
                   int32_t w_dtype, int64_t w_pitch, void* out, int32_t out_dtype, void* workspace, int64_t workspace_bytes, void* stream) {
-    if (int rc = check_product(a, b, out_dtype)) return rc;
+    tlb::MxProduct p{};
+    if (int rc = check_matmul(p, a, b, out, out_dtype, workspace, workspace_bytes)) return rc;
     if (x)
-        if (int rc = tlb_mx_quantize(a, x, x_dtype, x_pitch, stream)) return rc;
+        if (int rc = check_quantize(a, x, x_dtype, x_pitch)) return rc;
     if (w)
-        if (int rc = tlb_mx_quantize(b, w, w_dtype, w_pitch, stream)) return rc;
-    return tlb_mx_matmul(a, b, out, out_dtype, workspace, workspace_bytes, stream);
+        if (int rc = check_quantize(b, w, w_dtype, w_pitch)) return rc;
+    if (a->rows == 0 && b->rows == 0) return TLB_OK;
+    if (int rc = need_device()) return rc;
+    if (x && a->rows > 0)
+        if (int rc = quantize(*a, x, x_dtype, x_pitch, stream)) return rc;
+    if (w && b->rows > 0)
+        if (int rc = quantize(*b, w, w_dtype, w_pitch, stream)) return rc;
+    if (a->rows == 0 || b->rows == 0) return TLB_OK;
+    if (int e = tlb::launch_mx_matmul(p, stream)) return cuda_fail(e, "mx_linear");
+    return TLB_OK;
 }
 
 int tlb_mx_incomplete(uint32_t* count) {

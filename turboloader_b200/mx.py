@@ -111,7 +111,12 @@ def _rows_struct(codes, scales, rows, cols, fmt, scale):
 def _check_held(codes, scales, rows, cols, fmt):
     """codes (..., code pitch) and scales (..., scale pitch): uint8, contiguous, `rows` rows in all."""
     cp, sp = _pitches(fmt, cols)
-    for t, pitch, what in ((codes, cp, "codes"), (scales, sp, "scales")):
+    if (isinstance(codes, torch.Tensor) and isinstance(scales, torch.Tensor) and codes.is_cuda and codes.dtype is torch.uint8
+            and scales.dtype is torch.uint8 and codes.dim() and scales.dim() and codes.size(-1) == cp and scales.size(-1) == sp
+            and codes.numel() == rows * cp and scales.numel() == rows * sp and codes.get_device() == scales.get_device()
+            and codes.is_contiguous() and scales.is_contiguous() and not codes.data_ptr() % 16 and not scales.data_ptr() % 4):
+        return
+    for t, pitch, what in ((codes, cp, "codes"), (scales, sp, "scales")):  # what is wrong
         _cuda(t, what)
         if t.dtype is not torch.uint8 or not t.is_contiguous() or t.dim() < 1 or t.shape[-1] != pitch:
             raise ValueError(f"{what} must be a contiguous uint8 tensor with rows of {pitch} bytes")
