@@ -289,6 +289,39 @@ def test_product_scales_nan_rows_and_out(fmt, m):
         _close(got[:m - 1][:, keep], want[:m - 1][:, keep], magnitude[:m - 1][:, keep], k, torch.float32)
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("k", [300, 4100])
+def test_a_few_rows_are_the_first_rows_of_many(fmt, k):
+    """Each row's sums are its own: what other rows hold, or what ran before on the device, changes no bit of them."""
+    n, many = 330, 256
+    (a, av), (b, bv) = _held(many, k, fmt, 1, 3), _held(n, k, fmt, 2, 3)
+    whole = tb.mx_matmul(a, b, torch.float32)
+    _close(whole, av @ bv.T, av.abs() @ bv.abs().T, k, torch.float32)
+    nothing = tb.mx_quantize(torch.full((300, k), float("nan"), device="cuda"), fmt)
+    up = torch.randn(many, n, device="cuda")
+    for dtype in DTYPES:
+        x = torch.randn(many, k, device="cuda", dtype=dtype, requires_grad=True)
+        all_rows, = torch.autograd.grad(tb.mx_linear(x, b, fmt), [x], up.to(dtype))
+        for m in (5, 8, 9, 24, 31, 32, 33, 63, 127, 128, 129, 250):
+            part = tb.MxTensor(a.codes[:m], a.scales[:m], (m, k), fmt)
+            assert torch.isnan(tb.mx_matmul(nothing, nothing, torch.float32)).all()
+            assert torch.equal(tb.mx_matmul(part, b, torch.float32), whole[:m])
+            few = x.detach()[:m].requires_grad_(True)
+            lost = torch.full((m, n), float("nan"), device="cuda", dtype=dtype)
+            y = tb.mx_linear(few, b, fmt)
+            bad, = torch.autograd.grad(y, [few], lost, retain_graph=True)
+            rows, = torch.autograd.grad(y, [few], up.to(dtype)[:m])
+            assert torch.isnan(bad).all() and torch.equal(rows, all_rows[:m])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("m", [2, 3, 4])
+def test_two_to_four_rows_of_small_and_large_matrices(fmt, m):
+    for n, k in ((70, 40), (9000, 2048), (17000, 2048)):
+        (a, av), (b, bv) = _held(m, k, fmt, 1, 3), _held(n, k, fmt, 2, 3)
+        _close(tb.mx_matmul(a, b, torch.float32), av @ bv.T, av.abs() @ bv.abs().T, k, torch.float32)
+
+
 def test_product_of_nothing():
     x = torch.zeros(0, 64, device="cuda")
     w = tb.mx_quantize(torch.ones(5, 64, device="cuda"))

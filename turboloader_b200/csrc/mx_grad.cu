@@ -43,6 +43,7 @@ struct GradParams {
     long long sum;            // length of the sum, and stages of one term of it
     int term_stages, stages;  // stages: terms * term_stages
     int tile_n, m_tiles, n_tiles, splits;
+    int rows_a;               // rows of a copy of g: as rows_a of the product; 64 when g is transposed, in two copies
     int hold;                 // stages that an accumulator holds at most
     int transpose, scaled, vec_ok;
 };
@@ -108,7 +109,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
 
     if (warp == 0) {
         const bool issue = elect_one();
-        const unsigned full_at = at_leader(full), bytes = stage_bytes;
+        const unsigned full_at = at_leader(full), bytes = stage_bytes - kStageA + gp.rows_a * (gp.transpose ? 256u : 128u);
         Ring r;
         unsigned started = 0;
         bool ok = true;
@@ -411,6 +412,7 @@ GradParams plan(const MxGrad& p, const Shared& sh, bool of_b) {
     gp.sum = of_b ? p.m : p.n;
     gp.cols = gp.q.cols;
     gp.transpose = of_b;
+    gp.rows_a = of_b ? kDepth : mx_box_rows(gp.rows, kTileM);
     gp.term_stages = static_cast<int>((gp.sum + kDepth - 1) / kDepth);
     gp.stages = sh.terms * gp.term_stages;
     gp.m_tiles = static_cast<int>((gp.rows + 2 * kTileM - 1) / (2 * kTileM));
@@ -481,7 +483,7 @@ int one_grad(const MxGrad& p, const Shared& sh, bool of_b, const void* g, const 
     }
     GradParams gp = plan(p, sh, of_b);
     const unsigned long long g_rows = static_cast<unsigned long long>(sh.terms) * p.m;
-    if (int e = mx_encode_map(&gp.map_a, 2, g, p.n, g_rows, sh.g_pitch * 2ull, 64, gp.transpose ? kDepth : kTileM, 1)) return e;
+    if (int e = mx_encode_map(&gp.map_a, 2, g, p.n, g_rows, sh.g_pitch * 2ull, 64, gp.rows_a, 1)) return e;
     if (int e = mx_encode_map(&gp.map_b, 2, values, gp.cols, gp.q.rows, mx_padded(gp.cols) * 2ull, 64, kDepth, 1)) return e;
     if (gp.splits > 1) {
         const unsigned long long part_rows = static_cast<unsigned long long>(gp.m_tiles) * 2 * kTileM, row_bytes = static_cast<unsigned long long>(part_pitch(gp)) * 4;

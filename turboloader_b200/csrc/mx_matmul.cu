@@ -43,6 +43,7 @@ struct TileParams {
     int tile_n, n_tiles, groups_n;  // groups_n: groups of 128 rows that a tile's B scales take (1 or 2)
     long long m_tiles, tiles;
     int k_stages;
+    int rows_a;    // rows of A that a CTA copies for a stage: mx_box_rows
     int resident;  // A stays in shared memory over consecutive tiles of one row
     int vec_ok;    // output rows are multiples of 16 bytes: written by tensor-map copies
     int passing;   // the result is large for L2: its lines are the first to leave
@@ -203,7 +204,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
         const bool issue = elect_one();
         Ring r;
         unsigned rows = 0, started = 0;
-        const unsigned b_bytes = tile_n / 2 * 128 + kWords<FMT> * tp.groups_n * 512, a_bytes = kCodesA + kWords<FMT> * 512;
+        const unsigned b_bytes = tile_n / 2 * 128 + kWords<FMT> * tp.groups_n * 512, a_bytes = tp.rows_a * 128 + kWords<FMT> * 512;
         const unsigned full_at = at_leader(full), a_full_at = at_leader(a_full);
         int last_m = -1;
         bool ok = true;
@@ -396,6 +397,7 @@ void plan(TileParams& tp) {
     const int line = p.out_dtype == kF32 ? 32 : 64;
     tp.k_stages = (mx_code_pitch(p.a.format, p.a.cols) + 127) / 128;
     tp.resident = tp.k_stages <= kSlots;
+    tp.rows_a = mx_box_rows(p.a.rows, kTileM);
     for (int w = 16; w <= kMaxTileN; w += 16) {
         if (tp.resident && w % line && w < n && w > line) continue;
         const long long tiles = tp.m_tiles * ((n + w - 1) / w), cost = (tiles + kSms / 2 - 1) / (kSms / 2) * (w + 32);
@@ -467,7 +469,7 @@ int launch_mx_matmul(const MxProduct& p, void* stream) {
     tp.passing = out_pitch * p.a.rows > 64ll << 20;  // half of L2 (50176 x 4096 x 1024: 131 us without, 125 with)
     unsigned char* sa = static_cast<unsigned char*>(p.workspace);
     unsigned char* sb = sa + ga * 512;
-    if (int e = mx_encode_map(&tp.map_a, 1, p.a.codes, pitch, p.a.rows, pitch, 128, kTileM, 1)) return e;
+    if (int e = mx_encode_map(&tp.map_a, 1, p.a.codes, pitch, p.a.rows, pitch, 128, tp.rows_a, 1)) return e;
     if (int e = mx_encode_map(&tp.map_b, 1, p.b.codes, pitch, n, pitch, 128, tp.tile_n / 2, 1)) return e;
     if (int e = mx_encode_map(&tp.map_sa, 4, sa, 128, ga, 512, 128, words, 0)) return e;
     if (int e = mx_encode_map(&tp.map_sb, 4, sb, 128, gb, 512, 128, words * tp.groups_n, 0)) return e;
