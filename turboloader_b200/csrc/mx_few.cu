@@ -8,6 +8,8 @@
 // multiplied and summed in packed fp16, exactly: a half of a pair sums 8 products of at most 36 that are
 // multiples of 1/4, at most 1152 quarters, and fp16 holds 2048.  Every 16 products the sum goes to fp32,
 // times the two scales.  8-bit codes are multiplied in fp32.
+#include <algorithm>
+
 #include "mx_device.cuh"
 
 namespace tlb {
@@ -142,11 +144,15 @@ void by_format(const MxProduct& p, cudaStream_t st) {
 
 }  // namespace
 
-// With one or two rows reading bounds either way, and this kernel starts sooner; with three or four its
-// arithmetic grows, and only a small matrix is done sooner than by the tensor cores (4 rows: 4096 x 4096
-// 7.0 us against 12, 16384 x 16384 73 against 53).
+// With one row reading bounds either way, and this kernel starts sooner.  With two to four its arithmetic grows
+// with the rows, per byte of codes more for the smaller ones, while the tensor cores' time does not; a row of B
+// costs as much as 1024 values at least.  us here and there, rows x N x K: nvfp4 2 x 8192 x 8192 12.1 / 14.8,
+// 3 x 8192 x 4096 9.9 / 10.3, 4 x 8192 x 4096 12.0 / 10.3, 2 x 16384 x 8192 20.8 / 18.3; mxfp4 4 x 4096 x 4096
+// 8.5 / 8.8, 3 x 8192 x 4096 12.2 / 9.4; mxfp8 3 x 4096 x 4096 10.8 / 11.3, 4 x 4096 x 4096 13.5 / 11.3.
 bool mx_few(const MxProduct& p) {
-    return p.a.rows <= 2 || (p.a.rows <= 4 && p.b.rows * p.a.cols <= 1ll << 25);
+    if (p.a.rows <= 1 || p.a.rows > 4) return p.a.rows <= 1;
+    const long long most = p.a.format == kNvfp4 ? 3ll << 25 : p.a.format == kMxfp4 ? 1ll << 26 : 3ll << 24;
+    return p.a.rows * p.b.rows * std::max(p.a.cols, 1024) <= most;
 }
 
 int launch_mx_few(const MxProduct& p, void* stream) {
