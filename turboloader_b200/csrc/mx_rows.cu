@@ -120,6 +120,9 @@ struct Raw {
                     asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
                                  : "l"(reinterpret_cast<const unsigned char*>(p) + 32 * j));
+                } else if (have <= 0) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = 0u;
                 } else {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {  // the row's end: value by value
@@ -271,18 +274,19 @@ __global__ void __launch_bounds__(kThreads, !ALIGNED ? 1 : sizeof(T) == 2 ? 5 : 
         long long to;
         int left, unit;
     };
-    auto fetch = [&](Work& w, unsigned u) {
+    auto fetch = [&](Work& w, unsigned u) {  // false: the warp has no row that is written
         const bool in = u < all;
         const unsigned r = in ? by_units(u) : 0u;
         w.unit = static_cast<int>(in ? u - r * units : 0u);
         w.to = !in ? -1 : p.index ? dest[r] : static_cast<long long>(row0 + r);
+        if (!__any_sync(0xffffffffu, w.to >= 0)) return false;
         const unsigned over = by_tokens(token0 + r), token = token0 + r - over * p.tokens;
         w.left = w.to >= 0 ? p.q.cols - w.unit * take : 0;
         w.x = static_cast<const T*>(p.in) + (sample0 + over) * p.sample_pitch + token * p.row_pitch + w.unit * take;
         w.raw.load(w.x, w.left);
+        return true;
     };
     auto finish = [&](Work& w) {
-        if (!__any_sync(0xffffffffu, w.to >= 0)) return;
         float t[take];
         w.raw.values(w.x, w.left, t);
         if (ts != 1.0f) {
@@ -313,8 +317,7 @@ __global__ void __launch_bounds__(kThreads, !ALIGNED ? 1 : sizeof(T) == 2 ? 5 : 
     };
     for (unsigned u0 = threadIdx.x; u0 - threadIdx.x < all; u0 += kThreads) {  // whole warps stay together: lanes 2i, 2i + 1 may share a block
         Work w;
-        fetch(w, u0);
-        finish(w);
+        if (fetch(w, u0)) finish(w);
     }
 }
 
