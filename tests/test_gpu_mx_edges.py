@@ -1,0 +1,42 @@
+"""The microscaled operators where a call is unlike the usual one: saved-tensor hooks, other streams, empty sides,
+far scales, long sums."""
+import pytest
+import torch
+from torch.utils.checkpoint import checkpoint
+
+import turboloader_b200 as tb
+
+pytestmark = pytest.mark.gpu
+
+FORMATS = ("nvfp4", "mxfp4", "mxfp8")
+DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+# ---- saved tensors that the node does not own --------------------------------------------------------------------
+
+def _on_host_and_back():
+    return torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.cuda())
+
+
+@pytest.mark.parametrize("how", ["hooks", "checkpoint"])
+@pytest.mark.parametrize("held", ["neither", "x", "weight"])
+@pytest.mark.parametrize("m,n,k", [(40, 72, 200), (3000, 64, 96), (64, 2000, 130)])
+def test_gradients_under_saved_tensor_hooks_and_checkpoints(how, held, m, n, k):
+    g = torch.Generator(device="cuda").manual_seed(m)
+    x, w, up = (torch.randn(*s, generator=g, device="cuda") for s in ((m, k), (n, k), (m, n)))
+    x, w = (tb.mx_quantize(x, "mxfp4") if held == "x" else x.requires_grad_(True)), (tb.mx_quantize(w, "mxfp4") if held == "weight" else w.requires_grad_(True))
+    leaves = [t for t in (x, w) if isinstance(t, torch.Tensor)]
+
+    def layer(*leaves):
+        a, b = x if held == "x" else leaves[0], w if held == "weight" else leaves[-1]
+        return tb.mx_linear(a, b, "mxfp4", dtype=torch.float32)
+
+    want = torch.autograd.grad(layer(*leaves), leaves, up)
+    for _ in range(3):
+        if how == "hooks":
+            with _on_host_and_back():
+                y = layer(*leaves)
+        else:
+            y = checkpoint(layer, *leaves, use_reentrant=False)
+        got = torch.autograd.grad(y, leaves, up)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

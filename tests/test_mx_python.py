@@ -1,0 +1,87 @@
+"""The Python layer of the microscaled operators, with the library's calls replaced: what lives while a kernel may
+read it.  Runs without a GPU."""
+import pytest
+import torch
+from torch.multiprocessing.reductions import StorageWeakRef
+from torch.utils.checkpoint import checkpoint
+
+from turboloader_b200 import mx
+
+
+class _Library:
+    """Takes the entry points' calls; ``on_grad(a, b, grad_a, grad_b)`` sees the operands of a gradient."""
+
+    def __init__(self):
+        self.on_grad = lambda *a: None
+
+    def tlb_mx_quantize(self, *a):
+        return 0
+
+    def tlb_mx_linear(self, *a):
+        return 0
+
+    def tlb_mx_matmul_workspace(self, *a):
+        return 0
+
+    def tlb_mx_grad_workspace(self, *a):
+        return 1 << 16
+
+    def tlb_mx_grad(self, g, g_dtype, m, n, a, b, grad_a, a_dtype, grad_b, b_dtype, *rest):
+        self.on_grad(a, b, grad_a, grad_b)
+        return 0
+
+
+@pytest.fixture
+def library(monkeypatch):
+    lib = _Library()
+    monkeypatch.setattr(mx._capi, "load", lambda: lib)
+    monkeypatch.setattr(mx, "_cuda", lambda t, what: t)
+    monkeypatch.setattr(mx, "_away", lambda device, stream: False)
+    monkeypatch.setattr(mx, "_raw_stream", lambda index: None)
+    return lib
+
+
+class _Watched:
+    """A context whose saved tensors are watched, not kept."""
+
+    def __init__(self, ctx, watched):
+        self._ctx, self._watched = ctx, watched
+
+    def __getattr__(self, name):
+        return getattr(self._ctx, name)
+
+    @property
+    def saved_tensors(self):
+        saved = self._ctx.saved_tensors
+        self._watched += [(StorageWeakRef(t.untyped_storage()), t.data_ptr(), t.data_ptr() + t.nbytes) for t in saved]
+        return saved
+
+
+@pytest.mark.parametrize("how", ["plain", "hooks", "checkpoint"])
+@pytest.mark.parametrize("held", [False, True])
+def test_saved_rows_live_until_the_gradients_are_launched(library, monkeypatch, how, held):
+    """Under hooks and checkpoints the node does not own what it unpacks: only the backward pass keeps it alive."""
+    x = torch.randn(6, 64, requires_grad=True)
+    w = torch.randn(5, 64, requires_grad=True)
+    q = mx.MxTensor(torch.zeros(6, 64, dtype=torch.uint8), torch.zeros(6, 8, dtype=torch.uint8), (6, 64), "nvfp4") if held else x
+    watched, launched = [], []
+    backward = mx._MxLinear.backward
+    monkeypatch.setattr(mx._MxLinear, "backward", staticmethod(lambda ctx, g: backward(_Watched(ctx, watched), g)))
+
+    def on_grad(a, b, grad_a, grad_b):
+        assert watched and not any(storage.expired() for storage, _, _ in watched)
+        for rows in (a, b):
+            if rows is not None:
+                assert all(any(low <= at < high for _, low, high in watched) for at in (rows.codes, rows.scales))
+        launched.append((a is not None, b is not None, bool(grad_a), bool(grad_b)))
+
+    library.on_grad = on_grad
+    if how == "checkpoint":
+        y = checkpoint(lambda w: mx.mx_linear(q, w, "nvfp4"), w, use_reentrant=False)
+    elif how == "hooks":
+        with torch.autograd.graph.saved_tensors_hooks(torch.clone, torch.clone):
+            y = mx.mx_linear(q, w, "nvfp4")
+    else:
+        y = mx.mx_linear(q, w, "nvfp4")
+    y.sum().backward()
+    assert launched == [(True, not held, not held, True)]

@@ -393,8 +393,9 @@ class _MxLinear(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        saved = list(ctx.saved_tensors)
-        base = saved.pop(0).data_ptr() if ctx.one else 0
+        saved = ctx.saved_tensors  # held to the end: under hooks and checkpoints nothing else keeps the rows alive
+        left = iter(saved)
+        base = next(left).data_ptr() if ctx.one else 0
         cols = ctx.x_shape[-1]
         ops = []
         for part in ctx.parts:
@@ -405,8 +406,8 @@ class _MxLinear(torch.autograd.Function):
             if count == 0:
                 c, s = base + c, base + s
             else:  # a held operand: one buffer, or its codes and its scales
-                c = saved.pop(0).data_ptr()
-                s = saved.pop(0).data_ptr() if count == 2 else c + rows * _pitches(ctx.fmt, cols)[0]
+                c = next(left).data_ptr()
+                s = next(left).data_ptr() if count == 2 else c + rows * _pitches(ctx.fmt, cols)[0]
             ops.append(_rows_struct(c, s, rows, cols, ctx.fmt, ts))
         if g.dim() != 2 or not g.is_contiguous():
             g = g.reshape(-1, g.shape[-1]).contiguous()
