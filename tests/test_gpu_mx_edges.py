@@ -40,3 +40,21 @@ def test_gradients_under_saved_tensor_hooks_and_checkpoints(how, held, m, n, k):
             y = checkpoint(layer, *leaves, use_reentrant=False)
         got = torch.autograd.grad(y, leaves, up)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---- empty sides -----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("lead", [(), (3,), (2, 3), (2, 0)])
+@pytest.mark.parametrize("n", [0, 5])
+def test_gradients_of_any_leading_dimensions_and_of_no_rows(lead, n):
+    x = torch.randn(*lead, 40, device="cuda", requires_grad=True)
+    w = torch.randn(n, 40, device="cuda", requires_grad=True)
+    y = tb.mx_linear(x, w, "mxfp8")
+    up = torch.randn(*lead, n, device="cuda")
+    gx, gw = torch.autograd.grad(y, [x, w], up)
+    xv, wv = (tb.mx_quantize(t.detach().reshape(-1, 40), "mxfp8").dequantize().double() for t in (x, w))
+    u = up.double().reshape(xv.shape[0], n)
+    assert y.shape == (*lead, n) and gx.shape == x.shape and gw.shape == w.shape
+    # sums of at most 6 terms of three bf16 parts each, fp32
+    assert ((gx.reshape(-1, 40).double() - u @ wv).abs() <= 24 * 2.0 ** -23 * (u.abs() @ wv.abs()) + 1e-38).all()
+    assert ((gw.double() - u.T @ xv).abs() <= 24 * 2.0 ** -23 * (u.T.abs() @ xv.abs()) + 1e-38).all()

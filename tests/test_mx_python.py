@@ -85,3 +85,14 @@ def test_saved_rows_live_until_the_gradients_are_launched(library, monkeypatch, 
         y = mx.mx_linear(q, w, "nvfp4")
     y.sum().backward()
     assert launched == [(True, not held, not held, True)]
+
+
+@pytest.mark.parametrize("lead", [(), (3,), (2, 3), (0,), (2, 0), (2, 1, 3)])
+@pytest.mark.parametrize("n", [0, 5])
+def test_gradients_of_any_leading_dimensions_and_of_no_rows(library, lead, n):
+    x = torch.randn(*lead, 40, requires_grad=True)
+    w = torch.randn(n, 40, requires_grad=True)
+    y = mx.mx_linear(x, w, "mxfp8")
+    assert y.shape == (*lead, n)
+    gx, gw = torch.autograd.grad(y, [x, w], torch.ones(*lead, n))
+    assert gx.shape == x.shape and gw.shape == w.shape

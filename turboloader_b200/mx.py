@@ -410,7 +410,7 @@ class _MxLinear(torch.autograd.Function):
                 s = next(left).data_ptr() if count == 2 else c + rows * _pitches(ctx.fmt, cols)[0]
             ops.append(_rows_struct(c, s, rows, cols, ctx.fmt, ts))
         if g.dim() != 2 or not g.is_contiguous():
-            g = g.reshape(-1, g.shape[-1]).contiguous()
+            g = g.reshape(math.prod(ctx.x_shape[:-1]), g.shape[-1]).contiguous()
         if g.data_ptr() % 16:
             g = g.clone()
         gx, gw = _grads(g, *ops, cols, *ctx.types)
