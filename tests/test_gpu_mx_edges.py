@@ -58,3 +58,47 @@ def test_gradients_of_any_leading_dimensions_and_of_no_rows(lead, n):
     # sums of at most 6 terms of three bf16 parts each, fp32
     assert ((gx.reshape(-1, 40).double() - u @ wv).abs() <= 24 * 2.0 ** -23 * (u.abs() @ wv.abs()) + 1e-38).all()
     assert ((gw.double() - u.T @ xv).abs() <= 24 * 2.0 ** -23 * (u.T.abs() @ xv.abs()) + 1e-38).all()
+
+
+# ---- writes of one cache on several streams ----------------------------------------------------------------------
+
+@pytest.mark.parametrize("wrapped", [False, True])
+def test_first_long_writes_of_a_cache_on_two_streams(wrapped):
+    """Different slots, nothing before them that would order the two: the first stream is kept busy, the second is not."""
+    slots, cols = 1200, 96
+    for round_ in range(4):
+        cache = tb.MxCache.empty(slots, 1, cols, "mxfp8")
+        if wrapped:
+            cache = tb.MxCache(cache.codes, cache.scales, cols, "mxfp8", status=cache.status)
+        x = torch.randn(slots, cols, device="cuda")
+        order = torch.randperm(slots, device="cuda")
+        parts = order[:600], order[600:]
+        first, second = torch.cuda.Stream(), torch.cuda.Stream()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(first):
+            torch.cuda._sleep(20_000_000)
+        for at, stream in zip(parts, (first, second)):
+            with torch.cuda.stream(stream):
+                rows = x[at]
+                cache.write(at, rows)
+        torch.cuda.synchronize()
+        assert torch.equal(cache.read(None, torch.float32).view(slots, cols), tb.mx_quantize(x, "mxfp8").dequantize())
+        assert cache.device_status() == 0
+
+
+def test_a_first_long_write_that_is_captured():
+    slots, cols = 700, 64
+    cache = tb.MxCache.empty(slots, 1, cols)
+    index, x = torch.arange(600, device="cuda"), torch.randn(600, 1, cols, device="cuda")
+    index[599] = 3                                      # named twice: the last one stays
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.write(index, x)
+    for _ in range(2):
+        x.mul_(2)
+        graph.replay()
+        want = tb.mx_quantize(x.view(600, cols)).dequantize()
+        got = cache.read(None, torch.float32).view(slots, cols)
+        assert torch.equal(got[:3], want[:3]) and torch.equal(got[3], want[599]) and torch.equal(got[4:599], want[4:599])
+        assert not got[599:].any()

@@ -1,5 +1,7 @@
 """The Python layer of the microscaled operators, with the library's calls replaced: what lives while a kernel may
 read it.  Runs without a GPU."""
+import ctypes as C
+
 import pytest
 import torch
 from torch.multiprocessing.reductions import StorageWeakRef
@@ -12,7 +14,11 @@ class _Library:
     """Takes the entry points' calls; ``on_grad(a, b, grad_a, grad_b)`` sees the operands of a gradient."""
 
     def __init__(self):
-        self.on_grad = lambda *a: None
+        self.on_grad = self.on_write = lambda *a: None
+
+    def tlb_mx_write(self, cache, *a):
+        self.on_write(cache)
+        return 0
 
     def tlb_mx_quantize(self, *a):
         return 0
@@ -96,3 +102,22 @@ def test_gradients_of_any_leading_dimensions_and_of_no_rows(library, lead, n):
     assert y.shape == (*lead, n)
     gx, gw = torch.autograd.grad(y, [x, w], torch.ones(*lead, n))
     assert gx.shape == x.shape and gw.shape == w.shape
+
+
+def test_the_claims_of_a_write_are_its_own(library):
+    """No write sees words that another one, on another stream, may be claiming or has yet to fill."""
+    cache = mx.MxCache(torch.zeros(700, 1, 64, dtype=torch.uint8), torch.zeros(700, 1, 8, dtype=torch.uint8), 40, "nvfp4")
+    seen = []
+
+    def on_write(c):
+        words = (C.c_int32 * 700).from_address(c.owner)
+        seen.append(list(words))
+        words[:] = [5] * 700
+
+    library.on_write = on_write
+    for n in (257, 600):
+        cache.write(torch.arange(n), torch.zeros(n, 1, 40))
+    assert seen == [[-1] * 700] * 2
+    library.on_write = lambda c: seen.append(c.owner)
+    cache.write(torch.arange(256), torch.zeros(256, 1, 40))
+    assert seen[-1] is None

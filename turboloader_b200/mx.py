@@ -462,7 +462,6 @@ class MxCache:
 
     def __init__(self, codes, scales, cols, format, *, lengths=None, scale=1.0, status=None):
         self._fmt = _format_id(format)
-        self._owner = None
         _cuda(codes, "codes")
         if codes.dim() != 3:
             raise ValueError("codes must be (slots, tokens, code pitch)")
@@ -491,17 +490,17 @@ class MxCache:
         """Status bits the kernels OR-ed so far (synchronises); 0 when every index and length was valid."""
         return 0 if self.status is None else int(self.status.item())
 
-    def _struct(self):
+    def _struct(self, owner=None):
         rows = _rows_struct(self.codes.data_ptr(), self.scales.data_ptr(), self.slots * self.tokens, self.cols, self._fmt, self.scale)
         return _capi.MxCache(rows, self.tokens, None if self.lengths is None else self.lengths.data_ptr(),
-                             None if self._owner is None else self._owner.data_ptr(),
-                             None if self.status is None else self.status.data_ptr())
+                             None if owner is None else owner.data_ptr(), None if self.status is None else self.status.data_ptr())
 
     def write(self, index, x, *, lengths=None, stream=None):
         """Quantises sample ``x[i]`` (tokens, cols) into slot ``index[i]`` (int64 CUDA tensor).  With ``lengths``
         (int32, for a cache that has lengths) only the first ``lengths[i]`` rows are read and written; the slot's
         other rows stay as they were.  Without, all rows are there.  A slot named twice takes the last of its
-        samples; an index outside the cache is skipped and reported in ``status``."""
+        samples; an index outside the cache is skipped and reported in ``status``.  Writes that overlap in time (on
+        several streams) must not name the same slot."""
         device = self.device
         _cuda(x, "x")
         if x.dim() == 2 and self.tokens == 1:
@@ -526,11 +525,9 @@ class MxCache:
         if _away(device, stream):
             with _there(device, stream):
                 return self.write(index, x, lengths=lengths)
-        if self._owner is None and n > _capi.MX_SCAN_SAMPLES:
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError(f"write more than {_capi.MX_SCAN_SAMPLES} samples once before the capture: the first such call allocates")
-            self._owner = torch.full((self.slots,), -1, dtype=torch.int32, device=device)
-        _capi.check(_capi.load().tlb_mx_write(self._struct(), index.data_ptr(), n, x.data_ptr(), dt, x.stride(1), x.stride(0),
+        # The claims of a long write are this call's own: writes on several streams share nothing but the rows.
+        owner = torch.full((max(self.slots, 1),), -1, dtype=torch.int32, device=device) if n > _capi.MX_SCAN_SAMPLES else None
+        _capi.check(_capi.load().tlb_mx_write(self._struct(owner), index.data_ptr(), n, x.data_ptr(), dt, x.stride(1), x.stride(0),
                                               None if lengths is None else lengths.data_ptr(), _raw_stream(device.index)))
 
     def _picked(self, index):
