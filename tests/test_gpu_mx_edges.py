@@ -102,3 +102,19 @@ def test_a_first_long_write_that_is_captured():
         got = cache.read(None, torch.float32).view(slots, cols)
         assert torch.equal(got[:3], want[:3]) and torch.equal(got[3], want[599]) and torch.equal(got[4:599], want[4:599])
         assert not got[599:].any()
+
+
+# ---- scales on the device that change --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_scales_on_the_device_may_change_after_the_forward_pass(fmt):
+    x, w = torch.randn(70, 96, device="cuda", requires_grad=True), torch.randn(50, 96, device="cuda", requires_grad=True)
+    up = torch.randn(70, 50, device="cuda")
+    want = torch.autograd.grad(tb.mx_linear(x, w, fmt, scale=0.5, weight_scale=0.25), [x, w], up)
+    sx, sw = torch.tensor([0.5], device="cuda"), torch.tensor([0.25], device="cuda")
+    y = tb.mx_linear(x, w, fmt, scale=sx, weight_scale=sw)
+    q = tb.mx_quantize(x.detach(), fmt, scale=sx)
+    sx.fill_(7), sw.fill_(9)
+    got = torch.autograd.grad(y, [x, w], up)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(q.dequantize(), tb.mx_quantize(x.detach(), fmt, scale=0.5).dequantize())

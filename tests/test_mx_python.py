@@ -23,6 +23,9 @@ class _Library:
     def tlb_mx_quantize(self, *a):
         return 0
 
+    def tlb_mx_read_codes(self, *a):
+        return 0
+
     def tlb_mx_linear(self, *a):
         return 0
 
@@ -121,3 +124,43 @@ def test_the_claims_of_a_write_are_its_own(library):
     library.on_write = lambda c: seen.append(c.owner)
     cache.write(torch.arange(256), torch.zeros(256, 1, 40))
     assert seen[-1] is None
+
+
+def _value(address):
+    return C.c_float.from_address(address).value
+
+
+def test_scales_on_the_device_are_those_of_the_forward_pass(library):
+    """A caller may change its tensor before the gradients: the rows were made with the old value."""
+    x, w = torch.randn(6, 64, requires_grad=True), torch.randn(5, 64, requires_grad=True)
+    sx, sw = torch.tensor([0.5]), torch.tensor(0.25)
+    y = mx.mx_linear(x, w, "nvfp4", scale=sx, weight_scale=sw)
+    sx.fill_(7), sw.fill_(9)
+    seen = []
+    library.on_grad = lambda a, b, *rest: seen.append((_value(a.scale_dev), _value(b.scale_dev)))
+    y.sum().backward()
+    assert seen == [(0.5, 0.25)]
+
+
+def test_a_held_scale_that_changed_before_the_gradients_is_refused(library):
+    scale = torch.tensor([0.5])
+    held = mx.MxTensor(torch.zeros(6, 64, dtype=torch.uint8), torch.zeros(6, 8, dtype=torch.uint8), (6, 64), "nvfp4", scale=scale)
+    w = torch.randn(5, 64, requires_grad=True)
+    seen = []
+    library.on_grad = lambda a, *rest: seen.append(_value(a.scale_dev))
+    mx.mx_linear(held, w, "nvfp4").sum().backward()
+    assert seen == [0.5]
+    y = mx.mx_linear(held, w, "nvfp4")
+    scale.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    assert seen == [0.5]
+
+
+def test_rows_made_with_a_scale_on_the_device_keep_its_value(library):
+    scale = torch.tensor([0.5])
+    q = mx.mx_quantize(torch.randn(6, 64), scale=scale)
+    cache = mx.MxCache(torch.zeros(3, 1, 64, dtype=torch.uint8), torch.zeros(3, 1, 8, dtype=torch.uint8), 64, "nvfp4", scale=scale)
+    batch = cache.read_mx(torch.arange(2))
+    scale.fill_(3)
+    assert float(q.scale) == float(batch.scale) == 0.5 and float(cache.scale) == 3

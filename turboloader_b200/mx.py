@@ -82,6 +82,11 @@ def _check_scale(scale, device):
     return scale
 
 
+def _own(scale):
+    """A scale that the caller cannot change any more: what the rows stand for depends on it as long as they live."""
+    return scale.clone() if isinstance(scale, torch.Tensor) else scale
+
+
 def _away(device, stream):
     """Whether a call for tensors of ``device`` has to change the current device or stream first."""
     return stream is not None or torch.cuda.current_device() != device.index
@@ -221,8 +226,8 @@ def _as_rows(x, what):
 def mx_quantize(x, format="nvfp4", *, scale=1.0, stream=None):
     """``x`` (..., cols), float32, bfloat16 or float16, as an ``MxTensor``.  The values of a row must be
     contiguous and the rows equally spaced (a slice of a wider matrix will do).  ``scale``: the tensor scale
-    that values are divided by first, a float or one float32 value on the device; a power of two loses
-    nothing.  For ``nvfp4``, ``max|x| / 2688`` rounded up to a power of two uses the range of its scales."""
+    that values are divided by first, a float or one float32 value on the device (copied: the result keeps the
+    value of this call); a power of two loses nothing.  For ``nvfp4``, ``max|x| / 2688`` rounded up to a power of two uses the range of its scales."""
     fmt = _format_id(format)
     rows, _, pitch = _as_rows(x, "x")
     dt = _dtype_id(x.dtype, "x")
@@ -231,7 +236,7 @@ def mx_quantize(x, format="nvfp4", *, scale=1.0, stream=None):
     if _away(device, stream):
         with _there(device, stream):
             return mx_quantize(x, format, scale=scale)
-    q = MxTensor._empty(tuple(x.shape), (rows,), format, fmt, scale, device)
+    q = MxTensor._empty(tuple(x.shape), (rows,), format, fmt, _own(scale), device)
     _capi.check(_capi.load().tlb_mx_quantize(q._struct(), x.data_ptr(), dt, pitch, _raw_stream(device.index)))
     return q
 
@@ -336,16 +341,17 @@ def _align(n):
     return (n + 255) & ~255
 
 
-def _linear(x, weight, held_x, held_w, fmt, scale, weight_scale, dtype):
+def _linear(x, weight, held_x, held_w, fmt, scale, weight_scale, dtype, kept=(False, False)):
     """The product of mx_linear, and where its operands' rows lie: (out, buffer of those quantised here or None, for each
-    operand (held one or None, offsets of codes and scales in the buffer, rows, scale))."""
+    operand (held one or None, offsets of codes and scales in the buffer, rows, scale)).  kept: whether the operand's
+    rows are needed after this call."""
     lib = _capi.load()
     device = (held_x if x is None else x).device
     shape = held_x.shape if x is None else x.shape
     cols = shape[-1]
     cp, sp = _pitches(fmt, cols)
     at, given, plans = 0, [], []
-    for t, q, s in ((x, held_x, scale), (weight, held_w, weight_scale)):
+    for t, q, s, keep in ((x, held_x, scale, kept[0]), (weight, held_w, weight_scale, kept[1])):
         if t is None:
             given += None, 0, 0
             plans.append((q, 0, 0, q._rows, q.scale))
@@ -354,7 +360,8 @@ def _linear(x, weight, held_x, held_w, fmt, scale, weight_scale, dtype):
         codes, scales = at, at + _align(rows * cp)
         at = scales + _align(rows * sp)
         given += t, _DTYPES[t.dtype], pitch
-        plans.append((None, codes, scales, rows, _check_scale(s, device)))
+        s = _check_scale(s, device)
+        plans.append((None, codes, scales, rows, _own(s) if keep else s))
     xt, xd, xp, wt, wd, wp = given
     dt = _DTYPES[dtype]
     buf = torch.empty(at, dtype=torch.uint8, device=device) if at else None
@@ -370,18 +377,22 @@ def _linear(x, weight, held_x, held_w, fmt, scale, weight_scale, dtype):
 
 class _MxLinear(torch.autograd.Function):
     """`ctx.parts`: where the operands' rows lie that the backward pass needs, as (0, offsets of codes and scales in the
-    first saved tensor, rows, scale); of a held operand the first number counts its saved tensors."""
+    first saved tensor, rows, scale); of a held operand the first number counts its saved tensors of rows, and a scale of
+    None is the saved tensor behind them."""
 
     @staticmethod
     def forward(ctx, x, weight, held_x, held_w, fmt, scale, weight_scale, dtype):
-        out, buf, plans = _linear(x, weight, held_x, held_w, fmt, scale, weight_scale, dtype)
         needs_x, needs_w = ctx.needs_input_grad[:2]
+        out, buf, plans = _linear(x, weight, held_x, held_w, fmt, scale, weight_scale, dtype, (needs_w, needs_x))
         keep, parts = [] if buf is None else [buf], []
         for (q, c, s, rows, ts), needed in zip(plans, (needs_w, needs_x)):  # the gradient of one needs the other's codes
             count = 0
             if q is not None and needed:
                 keep += q._tensors()
                 count = len(q._tensors())
+                if isinstance(ts, torch.Tensor):
+                    keep.append(ts)
+                    ts = None
             parts.append((count, c, s, rows, ts) if needed else None)
         ctx.save_for_backward(*keep)
         ctx.parts = parts
@@ -408,6 +419,7 @@ class _MxLinear(torch.autograd.Function):
             else:  # a held operand: one buffer, or its codes and its scales
                 c = next(left).data_ptr()
                 s = next(left).data_ptr() if count == 2 else c + rows * _pitches(ctx.fmt, cols)[0]
+                ts = next(left) if ts is None else ts
             ops.append(_rows_struct(c, s, rows, cols, ctx.fmt, ts))
         if g.dim() != 2 or not g.is_contiguous():
             g = g.reshape(math.prod(ctx.x_shape[:-1]), g.shape[-1]).contiguous()
@@ -424,8 +436,8 @@ def mx_linear(x, weight, format="nvfp4", *, scale=1.0, weight_scale=1.0, dtype=N
     are their tensor scales), or ``MxTensor`` of that format, used as they are (cached features, a frozen weight).
     Gradients flow to the float tensors, straight through their quantisation: ``dx = g @ values(weight)`` and
     ``dweight = g.T @ values(x)``, with every value of g entering whole, sums in fp32, in the operand's own type;
-    for the backward pass only the codes are kept.  An ``MxTensor`` must stay unchanged until then.  ``dtype``
-    (the result's): by default ``weight``'s, else ``x``'s, else bfloat16."""
+    for the backward pass only the codes are kept, and the tensor scales as they were.  An ``MxTensor`` and its scale
+    must stay unchanged until then.  ``dtype`` (the result's): by default ``weight``'s, else ``x``'s, else bfloat16."""
     fmt = _format_id(format)
     held_x, held_w = (t if isinstance(t, MxTensor) else None for t in (x, weight))
     for t, held, what in ((x, held_x, "x"), (weight, held_w, "weight")):
@@ -560,7 +572,7 @@ class MxCache:
         if _away(device, stream):
             with _there(device, stream):
                 return self.read_mx(index)
-        q = MxTensor._empty((n, self.tokens, self.cols), (n, self.tokens), self.format, self._fmt, self.scale, device)
+        q = MxTensor._empty((n, self.tokens, self.cols), (n, self.tokens), self.format, self._fmt, _own(self.scale), device)
         lengths = None if self.lengths is None else torch.empty(n, dtype=torch.int32, device=device)
         _capi.check(_capi.load().tlb_mx_read_codes(self._struct(), at, n, *q._at(), None if lengths is None else lengths.data_ptr(),
                                                    _raw_stream(device.index)))
