@@ -164,3 +164,23 @@ def test_rows_made_with_a_scale_on_the_device_keep_its_value(library):
     batch = cache.read_mx(torch.arange(2))
     scale.fill_(3)
     assert float(q.scale) == float(batch.scale) == 0.5 and float(cache.scale) == 3
+
+
+def test_forward_mode_is_refused_not_dropped(library):
+    x, w = torch.randn(6, 64), torch.randn(5, 64)
+    with torch.autograd.forward_ad.dual_level():
+        assert mx.mx_linear(x, w).shape == (6, 5)      # no tangent: an ordinary call
+        for a, b in ((torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)), w), (x, torch.autograd.forward_ad.make_dual(w, torch.ones_like(w)))):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError):
+                    mx.mx_linear(a, b)
+
+
+@pytest.mark.filterwarnings("ignore::DeprecationWarning")
+def test_tracing_is_refused():
+    def call(x):
+        mx._away(torch.device("cuda", 0), None)        # what every entry point asks before it allocates
+        return x
+
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(call, torch.ones(1))

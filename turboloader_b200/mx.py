@@ -89,6 +89,8 @@ def _own(scale):
 
 def _away(device, stream):
     """Whether a call for tensors of ``device`` has to change the current device or stream first."""
+    if torch._C._get_tracing_state() is not None:
+        raise RuntimeError("the microscaled operators cannot be traced: torch would record the memory they allocate, not what their kernels write")
     return stream is not None or torch.cuda.current_device() != device.index
 
 
@@ -437,7 +439,8 @@ def mx_linear(x, weight, format="nvfp4", *, scale=1.0, weight_scale=1.0, dtype=N
     Gradients flow to the float tensors, straight through their quantisation: ``dx = g @ values(weight)`` and
     ``dweight = g.T @ values(x)``, with every value of g entering whole, sums in fp32, in the operand's own type;
     for the backward pass only the codes are kept, and the tensor scales as they were.  An ``MxTensor`` and its scale
-    must stay unchanged until then.  ``dtype`` (the result's): by default ``weight``'s, else ``x``'s, else bfloat16."""
+    must stay unchanged until then.  Forward-mode tangents and tracing are refused.  ``dtype`` (the result's): by default
+    ``weight``'s, else ``x``'s, else bfloat16."""
     fmt = _format_id(format)
     held_x, held_w = (t if isinstance(t, MxTensor) else None for t in (x, weight))
     for t, held, what in ((x, held_x, "x"), (weight, held_w, "weight")):
@@ -460,7 +463,8 @@ def mx_linear(x, weight, format="nvfp4", *, scale=1.0, weight_scale=1.0, dtype=N
         with _there(device, None):
             return mx_linear(x, weight, format, scale=scale, weight_scale=weight_scale, dtype=dtype)
     args = (None if held_x is not None else x, None if held_w is not None else weight, held_x, held_w, fmt, scale, weight_scale, dtype)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:2]):
+    # within forward-mode differentiation too: autograd then refuses a tangent instead of dropping it
+    if torch.autograd.forward_ad._current_level >= 0 or torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:2]):
         return _MxLinear.apply(*args)
     return _linear(*args)[0]
 
