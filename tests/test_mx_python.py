@@ -184,3 +184,19 @@ def test_tracing_is_refused():
 
     with pytest.raises(RuntimeError, match="traced"):
         torch.jit.trace(call, torch.ones(1))
+
+
+@pytest.mark.parametrize("x_held,w_held,x_grad,w_grad", [(False, False, True, True), (False, False, True, False), (False, False, False, True),
+                                                         (True, False, False, True), (False, True, True, False)])
+def test_only_rows_that_the_gradients_read_are_saved(library, x_held, w_held, x_grad, w_grad):
+    """The input's gradient reads the weight's rows and the weight's gradient the input's."""
+    def operand(rows, held, grad):
+        if held:
+            return mx.MxTensor(torch.zeros(rows, 512, dtype=torch.uint8), torch.zeros(rows, 64, dtype=torch.uint8), (rows, 1024), "nvfp4")
+        return torch.randn(rows, 1024, requires_grad=grad)
+
+    saved = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: saved.append(t.nbytes) or t, lambda t: t):
+        mx.mx_linear(operand(2, x_held, x_grad), operand(3, w_held, w_grad), "nvfp4")
+    size = {2: 1024 + 256, 3: 1536 + 256} if not (x_held or w_held) else {2: 2 * 576, 3: 3 * 576}  # parts of a buffer start at multiples of 256
+    assert sum(saved) == (size[2] if w_grad else 0) + (size[3] if x_grad else 0)

@@ -344,37 +344,38 @@ def _align(n):
 
 
 def _linear(x, weight, held_x, held_w, fmt, scale, weight_scale, dtype, kept=(False, False)):
-    """The product of mx_linear, and where its operands' rows lie: (out, buffer of those quantised here or None, for each
-    operand (held one or None, offsets of codes and scales in the buffer, rows, scale)).  kept: whether the operand's
-    rows are needed after this call."""
+    """The product of mx_linear, and where its operands' rows lie: (out, buffer of the kept ones quantised here or None,
+    for each operand (held one or None, offsets of codes and scales in its buffer, rows, scale)).  kept: whether the
+    operand's rows are needed after this call; the others' memory is given back at its end."""
     lib = _capi.load()
     device = (held_x if x is None else x).device
     shape = held_x.shape if x is None else x.shape
     cols = shape[-1]
     cp, sp = _pitches(fmt, cols)
-    at, given, plans = 0, [], []
+    at, given, plans = [0, 0], [], []  # sizes of the two buffers: of rows that end with the call, of kept ones
     for t, q, s, keep in ((x, held_x, scale, kept[0]), (weight, held_w, weight_scale, kept[1])):
         if t is None:
             given += None, 0, 0
             plans.append((q, 0, 0, q._rows, q.scale))
             continue
         t, rows, pitch = _spaced(t)
-        codes, scales = at, at + _align(rows * cp)
-        at = scales + _align(rows * sp)
+        codes, scales = at[keep], at[keep] + _align(rows * cp)
+        at[keep] = scales + _align(rows * sp)
         given += t, _DTYPES[t.dtype], pitch
         s = _check_scale(s, device)
         plans.append((None, codes, scales, rows, _own(s) if keep else s))
     xt, xd, xp, wt, wd, wp = given
     dt = _DTYPES[dtype]
-    buf = torch.empty(at, dtype=torch.uint8, device=device) if at else None
-    base = 0 if buf is None else buf.data_ptr()
-    a, b = [q._struct() if q is not None else _rows_struct(base + c, base + s, rows, cols, fmt, ts) for q, c, s, rows, ts in plans]
+    bufs = [torch.empty(size, dtype=torch.uint8, device=device) if size else None for size in at]
+    bases = [0 if buf is None else buf.data_ptr() for buf in bufs]
+    a, b = [q._struct() if q is not None else _rows_struct(bases[keep] + c, bases[keep] + s, rows, cols, fmt, ts)
+            for (q, c, s, rows, ts), keep in zip(plans, kept)]
     out = torch.empty(*shape[:-1], plans[1][3], dtype=dtype, device=device)
     size = lib.tlb_mx_matmul_workspace(a, b, dt)
     ws = _workspace(size, device)
     _capi.check(lib.tlb_mx_linear(a, None if xt is None else xt.data_ptr(), xd, xp, b, None if wt is None else wt.data_ptr(), wd, wp,
                                   out.data_ptr(), dt, None if ws is None else ws.data_ptr(), size, _raw_stream(device.index)))
-    return out, buf, plans
+    return out, bufs[True], plans
 
 
 class _MxLinear(torch.autograd.Function):
