@@ -5,6 +5,7 @@ import torch
 from torch.utils.checkpoint import checkpoint
 
 import turboloader_b200 as tb
+from mx_reference import decode
 
 pytestmark = pytest.mark.gpu
 
@@ -118,3 +119,34 @@ def test_scales_on_the_device_may_change_after_the_forward_pass(fmt):
     got = torch.autograd.grad(y, [x, w], up)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert torch.equal(q.dequantize(), tb.mx_quantize(x.detach(), fmt, scale=0.5).dequantize())
+
+
+# ---- far scales ------------------------------------------------------------------------------------------------
+
+def _values(q):
+    """What an MxTensor stands for without its tensor scale, float64."""
+    return torch.from_numpy(decode(q.codes.cpu().numpy(), q.scales.cpu().numpy(), q.format, q.shape[-1])).cuda()
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "mxfp8"])
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 200])
+def test_products_of_very_large_and_very_small_rows(fmt, m):
+    """Rows near the end of fp32's range times a weight near its beginning, either way round: the products are ordinary."""
+    n, k = 150, 320
+    g = torch.Generator(device="cuda").manual_seed(m)
+    for large, small in ((2.0 ** 120, 2.0 ** -100), (2.0 ** -110, 2.0 ** 124), (2.0 ** -126, 2.0 ** 123), (2.0 ** 60, 2.0 ** -60)):
+        a, b = (tb.mx_quantize(torch.rand(r, k, generator=g, device="cuda") * s, fmt) for r, s in ((m, large), (n, small)))
+        av, bv = _values(a), _values(b)
+        want = av @ bv.T
+        got = tb.mx_matmul(a, b, torch.float32)
+        assert torch.isfinite(got).all()
+        assert ((got.double() - want).abs() <= (k + 2) * 2.0 ** -23 * want).all()      # no value is negative
+    for at in (0, k - 1):                               # a block of NaN beside scales of any size
+        x = torch.rand(m, k, generator=g, device="cuda") * 2.0 ** -126
+        x[m - 1, at] = float("nan")
+        got = tb.mx_matmul(tb.mx_quantize(x, fmt), b, torch.float32)
+        assert torch.isnan(got[m - 1]).all() and torch.isfinite(got[:m - 1]).all()
+        w = torch.rand(n, k, generator=g, device="cuda") * 2.0 ** -126
+        w[7, at] = float("inf")
+        got = tb.mx_matmul(a, tb.mx_quantize(w, fmt), torch.float32)
+        assert torch.isnan(got[:, 7]).all() and torch.isfinite(got[:, 8:]).all() and torch.isfinite(got[:, :7]).all()
