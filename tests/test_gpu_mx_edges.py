@@ -150,3 +150,46 @@ def test_products_of_very_large_and_very_small_rows(fmt, m):
         w[7, at] = float("inf")
         got = tb.mx_matmul(a, tb.mx_quantize(w, fmt), torch.float32)
         assert torch.isnan(got[:, 7]).all() and torch.isfinite(got[:, 8:]).all() and torch.isfinite(got[:, :7]).all()
+
+
+# ---- long sums -------------------------------------------------------------------------------------------------
+
+def _check_long_sum(got, want, magnitude, stages):
+    """An accumulator holds 8 stages of 4 instructions (16-bit results: 32), each of which may cut 2^-23 of the partial
+    sum; the accumulators, and the parts of a split sum (74 at most, not less than 16 stages each), are added rounding to
+    nearest.  Beside it half a step of the result's type."""
+    hold = 8 if got.dtype == torch.float32 else 32
+    parts = stages / 8 + min(74, stages / 16)
+    bound = torch.finfo(got.dtype).eps / 2 * want.abs() + (4 * hold + parts + 4) * 2.0 ** -23 * magnitude
+    assert torch.isfinite(got).all() and ((got.double() - want).abs() <= bound).all(), float(((got.double() - want).abs() / bound).max())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("positive", [False, True])
+@pytest.mark.parametrize("m,n,k", [(64, 96, 20000), (300, 520, 60000), (257, 130, 5001), (3, 40, 70000)])
+def test_products_of_long_rows(fmt, positive, m, n, k):
+    g = torch.Generator(device="cuda").manual_seed(k)
+    draw = (lambda r: torch.rand(r, k, generator=g, device="cuda")) if positive else (lambda r: torch.randn(r, k, generator=g, device="cuda"))
+    a, b = tb.mx_quantize(draw(m), fmt), tb.mx_quantize(draw(n), fmt)
+    av, bv = a.dequantize().double(), b.dequantize().double()
+    for dtype in DTYPES:
+        _check_long_sum(tb.mx_matmul(a, b, dtype), av @ bv.T, av.abs() @ bv.abs().T, -(-k // (128 if fmt == "mxfp8" else 256)))
+
+
+@pytest.mark.parametrize("fmt,m,n,k", [("nvfp4", 3000, 2570, 1000), ("mxfp4", 300, 5000, 131), ("mxfp8", 5000, 130, 250), ("nvfp4", 20000, 1300, 1000),
+                                       ("mxfp4", 9000, 1027, 2045)])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("positive", [False, True])
+def test_gradients_of_long_sums(fmt, m, n, k, dtype, positive):
+    """Tiles of 128 and of 256 columns, more tiles than pairs of CTAs, either sum split and not, odd rows."""
+    g = torch.Generator(device="cuda").manual_seed(m)
+    draw = (lambda *s: torch.rand(*s, generator=g, device="cuda")) if positive else (lambda *s: torch.randn(*s, generator=g, device="cuda"))
+    x, w, up = (draw(*s).to(dtype) for s in ((m, k), (n, k), (m, n)))
+    x.requires_grad_(True), w.requires_grad_(True)
+    gx, gw = torch.autograd.grad(tb.mx_linear(x, w, fmt, dtype=dtype), [x, w], up)
+    xv, wv = (tb.mx_quantize(t.detach(), fmt).dequantize().double() for t in (x, w))
+    u, terms = up.double(), {torch.bfloat16: 1, torch.float16: 2, torch.float32: 3}[dtype]
+    _check_long_sum(gx, u @ wv, u.abs() @ wv.abs(), -(-n // 64) * terms)
+    _check_long_sum(gw, u.T @ xv, u.abs().T @ xv.abs(), -(-m // 64) * terms)
+    for wanted, value in ((x, gx), (w, gw)):              # one alone is made in the same way
+        assert torch.equal(torch.autograd.grad(tb.mx_linear(x, w, fmt, dtype=dtype), [wanted], up)[0], value)

@@ -10,10 +10,8 @@
 // The values, and g where it is transposed, lie with the sum across the rows: the instructions read them so
 // (the operand's other major order), 64 columns of 64 rows a box.  Roles of the warps as in the product:
 //   warp 0 copies, warp 1 (leader) issues, warps 4-11 write results while the next tile is being summed.
-// The tensor cores cut where they add to an accumulator, about 1e-8 of a sum for every 16 of its terms.  That
-// is below the rounding of a 16-bit result; a result of 32 bits (EXACT) takes the accumulators out every
-// kExactStages stages and adds them in registers, rounding to nearest (12544 x 1000 x 1024, g fp32: 7.4e-6 off
-// without it, 1.6e-7 with it).
+// Accumulators are taken out every hold_stages stages and added in registers, rounding to nearest (12544 x 1000 x 1024, g
+// fp32: 7.4e-6 off without it, 1.6e-7 with it).
 // With few tiles and a long sum, the sum is split; the parts go to a workspace in fp32 and add_kernel adds
 // them in order, so that the result does not depend on which part ends first.
 #include <atomic>
@@ -30,7 +28,6 @@ constexpr int kSmem = 1024 + kRing + 8 * kStaging;
 constexpr int kThreads = 384, kPairs = kSms / 2;
 static_assert(kSmem <= 227 * 1024 - 512, "shared memory");
 constexpr unsigned kTmemColumns = 512;
-constexpr int kExactStages = 8;
 
 __device__ unsigned g_gave_up;
 
@@ -44,7 +41,7 @@ struct GradParams {
     int term_stages, stages;  // stages: terms * term_stages
     int tile_n, m_tiles, n_tiles, splits;
     int rows_a;               // rows of a copy of g: as rows_a of the product; 64 when g is transposed, in two copies
-    int hold;                 // stages that an accumulator holds at most
+    int hold;                 // stages that an accumulator holds: hold_stages
     int transpose, scaled, vec_ok;
 };
 
@@ -68,7 +65,7 @@ struct Item {
     }
 };
 
-template <typename T, bool EXACT>
+template <typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_kernel(const __grid_constant__ GradParams gp) {
     extern __shared__ unsigned char raw[];
     __shared__ unsigned long long bars[2 * kMaxStages + 5];
@@ -201,46 +198,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
             const int n0 = item.n * gp.tile_n;
             const TileOut<T> to{&gp.map_out, static_cast<T*>(gp.out), gp.pitch, item.split * (static_cast<long long>(gp.m_tiles) * 2 * kTileM) + in_part,
                                 gp.splits > 1 ? 32 : static_cast<int>(min(32ll, gp.rows - in_part)), n0, min(gp.tile_n, gp.cols - n0), gp.vec_ok, policy};
-            if constexpr (!EXACT) {
+            TileSum<T> sum;
+            for (int from = item.first; from < item.last; from += gp.hold, ++count) {
                 const unsigned buf = count & 1;
                 ok = mbar_wait(acc_full + 8 * buf, (count >> 1) & 1, stop);
                 if (!ok) break;
                 tc_fence_after();
-                write_tile(to, lanes + buf * 256, gp.tile_n, half, lane, staging, alpha, acc_empty_at + 8 * buf);
-                ++count;
-            } else {
-                float sum[4][32];  // this warp's chunks, columns 32 half + 64 i ...
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int c = 0; c < 32; ++c) sum[i][c] = 0.0f;
-                for (int from = item.first; from < item.last; from += gp.hold, ++count) {
-                    const unsigned buf = count & 1;
-                    ok = mbar_wait(acc_full + 8 * buf, (count >> 1) & 1, stop);
-                    if (!ok) break;
-                    tc_fence_after();
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int c0 = half * 32 + i * 64;
-                        if (c0 >= gp.tile_n) continue;
-#pragma unroll
-                        for (int g = 0; g < 2; ++g) {
-                            unsigned v[16];
-                            tmem_load16(lanes + buf * 256 + c0 + g * 16, v);
-                            tmem_load_wait();
-#pragma unroll
-                            for (int c = 0; c < 16; ++c) sum[i][g * 16 + c] = __fadd_rn(sum[i][g * 16 + c], __uint_as_float(v[c]));
-                        }
-                    }
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_at(acc_empty_at + 8 * buf);
-                }
-                if (!ok) break;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (half * 32 + i * 64 < gp.tile_n) write_chunk(to, sum[i], half * 32 + i * 64, gp.tile_n, lane, staging, alpha);
+                sum.add(lanes + buf * 256, gp.tile_n, half, lane, acc_empty_at + 8 * buf);
             }
+            if (!ok) break;
+            sum.write(to, gp.tile_n, half, lane, staging, alpha);
         }
         if (lane == 0) tma_store_wait_read();
     }
@@ -433,7 +400,7 @@ GradParams plan(const MxGrad& p, const Shared& sh, bool of_b) {
             if (splits == 1) break;
         }
     }
-    gp.hold = (of_b ? p.grad_b_dtype : p.grad_a_dtype) == kF32 ? kExactStages : gp.stages;
+    gp.hold = hold_stages((of_b ? p.grad_b_dtype : p.grad_a_dtype) == kF32);
     return gp;
 }
 
@@ -442,14 +409,14 @@ size_t part_bytes(const GradParams& gp) {
     return gp.splits > 1 ? static_cast<size_t>(gp.splits) * gp.m_tiles * 2 * kTileM * part_pitch(gp) * 4 : 0;
 }
 
-template <typename T, bool EXACT>
+template <typename T>
 int launch_grad(const GradParams& gp, cudaStream_t st, bool after_operands) {
     static std::atomic<unsigned long long> prepared{0};  // one bit a device
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return last_error();
     const unsigned long long bit = 1ull << (dev & 63);
     if (!(prepared.load(std::memory_order_acquire) & bit)) {
-        const cudaError_t e = cudaFuncSetAttribute(grad_kernel<T, EXACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+        const cudaError_t e = cudaFuncSetAttribute(grad_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
         if (e != cudaSuccess) return static_cast<int>(e);
         prepared.fetch_or(bit, std::memory_order_release);
     }
@@ -464,7 +431,7 @@ int launch_grad(const GradParams& gp, cudaStream_t st, bool after_operands) {
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = after_operands ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, grad_kernel<T, EXACT>, gp);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, grad_kernel<T>, gp);
     if (e != cudaSuccess) return static_cast<int>(e);
     mx_count_launch();
     return last_error();
@@ -492,7 +459,7 @@ int one_grad(const MxGrad& p, const Shared& sh, bool of_b, const void* g, const 
         gp.scaled = 0;
         gp.vec_ok = 1;
         if (int e = mx_encode_map(&gp.map_out, 1, parts, row_bytes, gp.splits * part_rows, row_bytes, 128, 32, 1)) return e;
-        if (int e = sizeof(T) == 4 ? launch_grad<float, true>(gp, st, after_operands) : launch_grad<float, false>(gp, st, after_operands)) return e;
+        if (int e = launch_grad<float>(gp, st, after_operands)) return e;
         const long long part = static_cast<long long>(part_rows) * part_pitch(gp);
         if (gp.cols % 4 == 0)
             add_kernel<T, 4><<<blocks(gp.rows * (gp.cols / 4)), 256, 0, st>>>(gp, static_cast<const float*>(parts), part, part_pitch(gp), static_cast<T*>(result));
@@ -508,7 +475,7 @@ int one_grad(const MxGrad& p, const Shared& sh, bool of_b, const void* g, const 
     gp.vec_ok = row_bytes % 16 == 0;
     if (gp.vec_ok)
         if (int e = mx_encode_map(&gp.map_out, 1, result, row_bytes, gp.rows, row_bytes, 128, 32, 1)) return e;
-    return launch_grad<T, sizeof(T) == 4>(gp, st, after_operands);
+    return launch_grad<T>(gp, st, after_operands);
 }
 
 int typed_grad(const MxGrad& p, const Shared& sh, bool of_b, const void* g, const void* values, void* parts, bool after_operands, cudaStream_t st) {

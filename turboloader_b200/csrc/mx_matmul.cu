@@ -32,6 +32,7 @@ constexpr int kStages = 5, kStageBytes = kCodesA + kScaleA + kCodesB + kScaleB;
 constexpr int kSlots = 4, kSlotBytes = kCodesA + kScaleA, kStagesB = 6, kStageBBytes = kCodesB + kScaleB;
 constexpr int kRing = kSlots * kSlotBytes + kStagesB * kStageBBytes;
 static_assert(kStages * kStageBytes <= kRing && kStageBytes % 1024 == 0 && kSlotBytes % 1024 == 0 && kStageBBytes % 1024 == 0, "layout");
+static_assert(kSlots <= hold_stages(true) && kSlots <= hold_stages(false), "a resident tile's sum stays in one accumulator");
 constexpr int kSmem = 1024 + kRing + 8 * kStaging;
 constexpr int kThreads = 384;
 static_assert(kSmem <= 227 * 1024 - 512, "shared memory");
@@ -148,7 +149,8 @@ __global__ void __launch_bounds__(kArrangeThreads) arrange_kernel(Arrange a, Arr
 }
 
 // ---- products ------------------------------------------------------------------------------------------------
-template <typename T, int FMT>
+// LONG: sums of more stages than an accumulator holds; A is then never resident.
+template <typename T, int FMT, bool LONG>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ TileParams tp) {
     extern __shared__ unsigned char raw[];
     __shared__ unsigned long long bars[2 * kStagesB + 4 + 2 * kSlots + 1];
@@ -159,6 +161,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
     const unsigned rank = __shfl_sync(0xffffffffu, cluster_rank(), 0);
     const MxProduct& p = tp.p;
     const int tile_n = tp.tile_n;
+    constexpr int hold = hold_stages(sizeof(T) == 4);
     const unsigned ring = tp.resident ? kStagesB : kStages;
     // Where A and its scales lie (of stage s, or of slot kt), and where stage s keeps B and its scales.
     const unsigned a_base = smem, a_step = tp.resident ? kSlotBytes : kStageBytes;
@@ -265,7 +268,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
         unsigned count = 0, rows = 0;
         int last_m = -1;
         bool ok = true;
-        for (Walk w(tp); ok && w.tile < w.end; w.tile += w.step, ++count) {
+        for (Walk w(tp); ok && w.tile < w.end; w.tile += w.step) {
             int m, n;
             w.place(tp, m, n);
             const bool new_row = tp.resident && m != last_m;
@@ -275,37 +278,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
                 last_m = m;
                 ++rows;
             }
-            const unsigned buf = count & 1;
-            if (!mbar_wait(acc_empty + 8 * buf, ((count >> 1) & 1) ^ 1, stop)) break;
-            tc_fence_after();
-            const unsigned d = tmem + buf * kMaxTileN;
-            for (int kt = 0; kt < tp.k_stages; ++kt) {
-                ok = (!new_row || mbar_wait(a_full + 8 * kt, (rows - 1) & 1, stop)) && mbar_wait(full + 8 * r.s, r.parity, stop);
+            for (int from = 0; ok && from < tp.k_stages; from += hold, ++count) {
+                const unsigned buf = count & 1;
+                ok = mbar_wait(acc_empty + 8 * buf, ((count >> 1) & 1) ^ 1, stop);
                 if (!ok) break;
                 tc_fence_after();
-                const unsigned a = a_base + (tp.resident ? kt : r.s) * a_step, b = b_base + r.s * b_step;
-                const unsigned sa = a + kCodesA, sb = b + kCodesB;
-                const unsigned long long da = smem_desc(a, 16, 1024, 2), db = smem_desc(b, 16, 1024, 2);
-                if (issue) {
+                const unsigned d = tmem + buf * kMaxTileN;
+                const int to = LONG ? min(from + hold, tp.k_stages) : tp.k_stages;
+                for (int kt = from; kt < to; ++kt) {
+                    ok = (!new_row || mbar_wait(a_full + 8 * kt, (rows - 1) & 1, stop)) && mbar_wait(full + 8 * r.s, r.parity, stop);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const unsigned a = a_base + (tp.resident ? kt : r.s) * a_step, b = b_base + r.s * b_step;
+                    const unsigned sa = a + kCodesA, sb = b + kCodesB;
+                    const unsigned long long da = smem_desc(a, 16, 1024, 2), db = smem_desc(b, 16, 1024, 2);
+                    if (issue) {
 #pragma unroll
-                    for (int g = 0; g < kWords<FMT>; ++g) {
-                        copy_scales(tmem + kTmemScaleA + 4 * g, sa + 512 * g);
-                        copy_scales(tmem + kTmemScaleB + 8 * g, sb + 512 * g * tp.groups_n);
-                        if (tp.groups_n > 1) copy_scales(tmem + kTmemScaleB + 8 * g + 4, sb + 1024 * g + 512);
-                    }
+                        for (int g = 0; g < kWords<FMT>; ++g) {
+                            copy_scales(tmem + kTmemScaleA + 4 * g, sa + 512 * g);
+                            copy_scales(tmem + kTmemScaleB + 8 * g, sb + 512 * g * tp.groups_n);
+                            if (tp.groups_n > 1) copy_scales(tmem + kTmemScaleB + 8 * g + 4, sb + 1024 * g + 512);
+                        }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int g = i * kWords<FMT> / 4;                                          // group of 4 scales
-                        const unsigned id = FMT == kNvfp4 ? 0u : FMT == kMxfp4 ? (i & 1) * 2u : i;  // first scale of it
-                        mma<FMT>(d, da + 2 * i, db + 2 * i, idesc | id << 4 | id << 29, tmem + kTmemScaleA + 4 * g, tmem + kTmemScaleB + 8 * g,
-                                 kt > 0 || i > 0);
+                        for (int i = 0; i < 4; ++i) {
+                            const int g = i * kWords<FMT> / 4;                                          // group of 4 scales
+                            const unsigned id = FMT == kNvfp4 ? 0u : FMT == kMxfp4 ? (i & 1) * 2u : i;  // first scale of it
+                            mma<FMT>(d, da + 2 * i, db + 2 * i, idesc | id << 4 | id << 29, tmem + kTmemScaleA + 4 * g, tmem + kTmemScaleB + 8 * g,
+                                     kt > from || i > 0);
+                        }
+                        tc_commit(empty + 8 * r.s);
+                        if (row_ends) tc_commit(a_empty + 8 * kt);
+                        if (kt == to - 1) tc_commit(acc_full + 8 * buf);
                     }
-                    tc_commit(empty + 8 * r.s);
-                    if (row_ends) tc_commit(a_empty + 8 * kt);
-                    if (kt == tp.k_stages - 1) tc_commit(acc_full + 8 * buf);
+                    __syncwarp();
+                    r.next(ring);
                 }
-                __syncwarp();
-                r.next(ring);
             }
         }
         if (*stop) {  // the instructions issued so far are done before TMEM is freed
@@ -322,18 +329,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
         const unsigned acc_empty_at = at_leader(acc_empty);
         const unsigned long long policy = store_policy(tp.passing);
         unsigned count = 0;
-        for (Walk w(tp); w.tile < w.end; w.tile += w.step, ++count) {
+        const unsigned lanes = tmem + (static_cast<unsigned>(quarter * 32) << 16);
+        bool ok = true;
+        for (Walk w(tp); ok && w.tile < w.end; w.tile += w.step) {
             int m, n;
             w.place(tp, m, n);
-            const unsigned buf = count & 1;
-            if (!mbar_wait(acc_full + 8 * buf, (count >> 1) & 1, stop)) break;
-            tc_fence_after();
             const long long m0 = static_cast<long long>(2 * m + rank) * kTileM + quarter * 32;
             const int n0 = n * tile_n;
             const TileOut<T> to{&tp.map_out, static_cast<T*>(p.out), n_all, m0, static_cast<int>(min(32ll, p.a.rows - m0)), n0, min(tile_n, n_all - n0),
                                 tp.vec_ok, policy};
-            write_tile(to, tmem + (static_cast<unsigned>(quarter * 32) << 16) + buf * kMaxTileN, tile_n, half, lane, staging, alpha,
-                       acc_empty_at + 8 * buf);
+            if constexpr (LONG) {
+                TileSum<T> sum;
+                for (int from = 0; from < tp.k_stages; from += hold, ++count) {
+                    const unsigned buf = count & 1;
+                    ok = mbar_wait(acc_full + 8 * buf, (count >> 1) & 1, stop);
+                    if (!ok) break;
+                    tc_fence_after();
+                    sum.add(lanes + buf * kMaxTileN, tile_n, half, lane, acc_empty_at + 8 * buf);
+                }
+                if (ok) sum.write(to, tile_n, half, lane, staging, alpha);
+            } else {
+                const unsigned buf = count & 1;
+                ok = mbar_wait(acc_full + 8 * buf, (count >> 1) & 1, stop);
+                if (!ok) break;
+                tc_fence_after();
+                write_tile(to, lanes + buf * kMaxTileN, tile_n, half, lane, staging, alpha, acc_empty_at + 8 * buf);
+                ++count;
+            }
         }
         if (lane == 0) tma_store_wait_read();
     }
@@ -348,14 +370,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
 
 int last_error() { return static_cast<int>(cudaGetLastError()); }
 
-template <typename T, int FMT>
+template <typename T, int FMT, bool LONG>
 int launch_tiles(const TileParams& tp, cudaStream_t st) {
     static std::atomic<unsigned long long> prepared{0};  // one bit a device
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return last_error();
     const unsigned long long bit = 1ull << (dev & 63);
     if (!(prepared.load(std::memory_order_acquire) & bit)) {
-        const cudaError_t e = cudaFuncSetAttribute(product_kernel<T, FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+        const cudaError_t e = cudaFuncSetAttribute(product_kernel<T, FMT, LONG>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
         if (e != cudaSuccess) return static_cast<int>(e);
         prepared.fetch_or(bit, std::memory_order_release);
     }
@@ -369,7 +391,7 @@ int launch_tiles(const TileParams& tp, cudaStream_t st) {
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, product_kernel<T, FMT>, tp);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, product_kernel<T, FMT, LONG>, tp);
     if (e != cudaSuccess) return static_cast<int>(e);
     mx_count_launch();
     return last_error();
@@ -377,9 +399,10 @@ int launch_tiles(const TileParams& tp, cudaStream_t st) {
 
 template <typename T>
 int by_format(const TileParams& tp, cudaStream_t st) {
-    if (tp.p.a.format == kNvfp4) return launch_tiles<T, kNvfp4>(tp, st);
-    if (tp.p.a.format == kMxfp4) return launch_tiles<T, kMxfp4>(tp, st);
-    return launch_tiles<T, kMxfp8>(tp, st);
+    const bool more = tp.k_stages > hold_stages(sizeof(T) == 4);
+    if (tp.p.a.format == kNvfp4) return more ? launch_tiles<T, kNvfp4, true>(tp, st) : launch_tiles<T, kNvfp4, false>(tp, st);
+    if (tp.p.a.format == kMxfp4) return more ? launch_tiles<T, kMxfp4, true>(tp, st) : launch_tiles<T, kMxfp4, false>(tp, st);
+    return more ? launch_tiles<T, kMxfp8, true>(tp, st) : launch_tiles<T, kMxfp8, false>(tp, st);
 }
 
 int words_of(int fmt) { return fmt == kNvfp4 ? 4 : fmt == kMxfp4 ? 2 : 1; }
