@@ -364,7 +364,8 @@ TLB_API void tlb_epoch_destroy(tlb_epoch* e);
  *   TLB_MX_MXFP8  32 values: scale s = 2^max(floor(log2 a) - 8, -127), codes e4m3(t / s)
  * An nvfp4 scale that rounds to zero makes its codes zero.  A block that holds an infinity or a NaN
  * gets a NaN scale and zero codes: all of it reads as NaN.  A code stands for code * s * tensor scale
- * (code * s is exact in fp32 and in bf16).
+ * (code * s is exact in fp32, and in bf16 where it is a multiple of bf16's least subnormal 2^-133: always but for
+ * mxfp8 blocks of values under 2^-118).
  *
  * Layout: rows are padded to 128 values; a row of codes takes tlb_mx_code_pitch bytes (4-bit codes: two a
  * byte, the earlier value in the low half) and a row of scales tlb_mx_scale_pitch bytes, rows packed
@@ -442,7 +443,7 @@ TLB_API int tlb_mx_incomplete(uint32_t* count);
 /* Gradients of that product with respect to the values of its operands, g (m, n) packed:
  *   grad_a (m, cols) = g * values(b)        grad_b (n, cols) = g^T * values(a)
  * grad_a or grad_b may be NULL (not wanted), and then b or a too.  Every value of g enters whole (fp32 as the
- * sum of three bf16 terms, fp16 of two); sums in fp32.  workspace as above, tlb_mx_grad_workspace bytes (which
+ * sum of three bf16 terms, fp16 of two; what an fp32 value has below 2^-133 is dropped); sums in fp32.  workspace as above, tlb_mx_grad_workspace bytes (which
  * looks at grad_a and grad_b for NULL alone). */
 TLB_API int64_t tlb_mx_grad_workspace(int32_t g_dtype, int64_t m, int64_t n, const tlb_mx_rows* a, const tlb_mx_rows* b,
                                       const void* grad_a, int32_t grad_a_dtype, const void* grad_b, int32_t grad_b_dtype);

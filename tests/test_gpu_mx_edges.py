@@ -152,6 +152,23 @@ def test_products_of_very_large_and_very_small_rows(fmt, m):
         assert torch.isnan(got[:, 7]).all() and torch.isfinite(got[:, 8:]).all() and torch.isfinite(got[:, :7]).all()
 
 
+@pytest.mark.parametrize("fmt", FORMATS[1:])
+@pytest.mark.parametrize("e", [-110, -118, -122, -128, -131])
+def test_gradients_of_very_small_values(fmt, e):
+    """bf16 ends at 2^-133: less than that is lost of a value of the weight, or of the gradient's fp32."""
+    m, n, k = 200, 64, 96
+    g = torch.Generator(device="cuda").manual_seed(-e)
+    x = torch.randn(m, k, generator=g, device="cuda", requires_grad=True)
+    for w_exponent, up_exponent in ((e, 60), (60, e)):
+        q = tb.mx_quantize(torch.randn(n, k, generator=g, device="cuda") * 2.0 ** w_exponent, fmt)
+        up = torch.randn(m, n, generator=g, device="cuda") * 2.0 ** up_exponent
+        got, = torch.autograd.grad(tb.mx_linear(x, q, fmt), [x], up)
+        w, u = q.dequantize().double(), up.double()
+        lost = u.abs().sum(1, keepdim=True) if w_exponent == e else w.abs().sum(0, keepdim=True)
+        # 3 stages of 4 instructions, and the values
+        assert ((got.double() - u @ w).abs() <= 2.0 ** -133 * lost + 16 * 2.0 ** -23 * (u.abs() @ w.abs()) + 2.0 ** -149).all()
+
+
 # ---- long sums -------------------------------------------------------------------------------------------------
 
 def _check_long_sum(got, want, magnitude, stages):

@@ -4,7 +4,9 @@
 // Both are products of bf16 matrices on the tensor cores.  code * block scale has at most 8 significant bits, so
 // operands_kernel writes the values as bf16 without a rounding (the tensor's scale is alpha).  g enters whole
 // too: bf16 as it is, fp16 as the sum of 2 and fp32 of 3 bf16 terms of 8 bits each, whose products are summed in
-// the same accumulators, the terms being further stages of the sum.
+// the same accumulators, the terms being further stages of the sum.  Both as far as bf16 reaches down: its least
+// subnormal is 2^-133.  What lies below it of an fp32 g (whole from 2^-110 on) is dropped, and the smallest codes of
+// mxfp8 blocks whose largest value is under 2^-118 are rounded to it: less than 2^-133 a value either way.
 //
 // grad_kernel: a pair of CTAs (a cluster of 2) makes output tiles of 256 x tile_n, 64 of the sum a stage.
 // The values, and g where it is transposed, lie with the sum across the rows: the instructions read them so

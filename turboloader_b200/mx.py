@@ -438,7 +438,7 @@ def mx_linear(x, weight, format="nvfp4", *, scale=1.0, weight_scale=1.0, dtype=N
     ``x`` and ``weight`` are float tensors, quantised to ``format`` by this call (``scale`` and ``weight_scale``
     are their tensor scales), or ``MxTensor`` of that format, used as they are (cached features, a frozen weight).
     Gradients flow to the float tensors, straight through their quantisation: ``dx = g @ values(weight)`` and
-    ``dweight = g.T @ values(x)``, with every value of g entering whole, sums in fp32, in the operand's own type;
+    ``dweight = g.T @ values(x)``, with every value of g entering whole (down to 2^-133), sums in fp32, in the operand's own type;
     for the backward pass only the codes are kept, and the tensor scales as they were.  An ``MxTensor`` and its scale
     must stay unchanged until then.  Forward-mode tangents and tracing are refused.  ``dtype`` (the result's): by default
     ``weight``'s, else ``x``'s, else bfloat16."""
