@@ -414,7 +414,8 @@ typedef struct tlb_mx_cache {
 TLB_API int tlb_mx_write(const tlb_mx_cache* cache, const int64_t* index, int64_t n, const void* x, int32_t x_dtype,
                          int64_t row_pitch, int64_t sample_pitch, const int32_t* lengths, void* stream);
 /* Samples index[i] (NULL: 0..n-1) as values, (n, tokens, cols) packed: zeros behind a sample's length
- * and for an index outside the cache (TLB_DEV_BAD_INDEX).  lengths_out (may be NULL): their lengths. */
+ * and for an index outside the cache (TLB_DEV_BAD_INDEX).  lengths_out (may be NULL): their lengths; one that the
+ * caller put into the cache outside [0, tokens] is clamped and reported (TLB_DEV_BAD_LENGTH). */
 TLB_API int tlb_mx_read(const tlb_mx_cache* cache, const int64_t* index, int64_t n, void* out, int32_t out_dtype,
                         int32_t* lengths_out, void* stream);
 /* The same samples as they are held: codes and scales of n * tokens rows, zero rows where tlb_mx_read

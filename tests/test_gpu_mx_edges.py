@@ -105,6 +105,22 @@ def test_a_first_long_write_that_is_captured():
         assert not got[599:].any()
 
 
+def test_lengths_of_a_cache_that_are_out_of_range_are_clamped_and_reported():
+    tokens, cols = 3, 40
+    for bad, size in ((tokens + 2, tokens), (-1, 0)):
+        cache = tb.MxCache.empty(5, tokens, cols, ragged=True)
+        cache.write(torch.arange(5, device="cuda"), torch.randn(5, tokens, cols, device="cuda"))
+        cache.lengths[2] = bad
+        for read in (cache.read, cache.read_mx):
+            values, lengths = read(torch.tensor([0, 1], device="cuda"))
+            assert cache.device_status() == 0
+            values, lengths = read(torch.tensor([1, 2], device="cuda"))
+            assert lengths.tolist() == [tokens, size] and cache.device_status() == 16
+            values = values.dequantize() if isinstance(values, tb.MxTensor) else values
+            assert bool(values[1].any()) == (size > 0)
+            cache.status.zero_()
+
+
 # ---- scales on the device that change --------------------------------------------------------------------------
 
 @pytest.mark.parametrize("fmt", FORMATS)
