@@ -200,3 +200,40 @@ def test_only_rows_that_the_gradients_read_are_saved(library, x_held, w_held, x_
         mx.mx_linear(operand(2, x_held, x_grad), operand(3, w_held, w_grad), "nvfp4")
     size = {2: 1024 + 256, 3: 1536 + 256} if not (x_held or w_held) else {2: 2 * 576, 3: 3 * 576}  # parts of a buffer start at multiples of 256
     assert sum(saved) == (size[2] if w_grad else 0) + (size[3] if x_grad else 0)
+
+
+# ---- the loader --------------------------------------------------------------------------------------------------
+
+class _Images:
+    """What a feature loader sees of an image loader."""
+
+    def __init__(self, n, batch_size, items, **kw):
+        self._n, self.batch_size, self._items = n, batch_size, items
+        self.__dict__.update(kw)
+
+    def __iter__(self):
+        return iter(self._items)
+
+
+def _feature_loader(monkeypatch):
+    from turboloader_b200 import CudaFeatureLoader
+
+    loader = CudaFeatureLoader.__new__(CudaFeatureLoader)
+    loader._torch, loader._device, loader._n = torch, torch.device("cpu"), 100
+    written = []
+    monkeypatch.setattr(loader, "write", lambda indices, features, lengths=None: written.append((list(indices), features, lengths)), raising=False)
+    return loader, written
+
+
+def test_fill_refuses_loaders_that_leave_samples_out(monkeypatch):
+    loader, written = _feature_loader(monkeypatch)
+    batch = (torch.zeros(4, 3), [0, 1, 2, 3])
+    with pytest.raises(ValueError, match="last 2 of its 10"):
+        loader.fill(_Images(10, 4, [batch, batch], drop_last=True, return_indices=True), lambda x: x)
+    with pytest.raises(ValueError, match="return_indices"):   # images and labels
+        loader.fill(_Images(8, 4, [batch, batch], drop_last=True, return_indices=False), lambda x: x)
+    assert not written
+    for images in (_Images(10, 4, [batch, batch], drop_last=False, return_indices=True), _Images(8, 4, [batch, batch], drop_last=True, return_indices=True),
+                   [batch, batch]):
+        assert loader.fill(images, lambda x: x) == 8
+    assert len(written) == 6

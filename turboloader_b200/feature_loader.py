@@ -64,8 +64,14 @@ class CudaFeatureLoader:
     def fill(self, batches, encoder):
         """Runs ``encoder`` over an image loader that was made with ``return_indices=True`` (``CudaResidentLoader``)
         and stores what it returns: features (n, tokens, dim), or ``(features, lengths)``.  The images reach the
-        encoder as CUDA tensors.  Returns the number of samples written."""
+        encoder as CUDA tensors.  Returns the number of samples written.  A loader that leaves out its last, smaller
+        batch is refused: those samples would read as zeros."""
         torch = self._torch
+        if getattr(batches, "return_indices", True) is False:  # its second item would be labels
+            raise ValueError("fill needs batches with indices (return_indices=True)")
+        samples = getattr(batches, "_n", None)
+        if getattr(batches, "drop_last", False) and samples is not None and samples % batches.batch_size:
+            raise ValueError(f"the loader drops the last {samples % batches.batch_size} of its {samples} samples: make it with drop_last=False")
         written = 0
         with torch.no_grad():
             for items in batches:
