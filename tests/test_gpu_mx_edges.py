@@ -1,5 +1,6 @@
 """The microscaled operators where a call is unlike the usual one: saved-tensor hooks, other streams, empty sides,
 far scales, long sums."""
+import numpy as np
 import pytest
 import torch
 from torch.utils.checkpoint import checkpoint
@@ -119,6 +120,29 @@ def test_lengths_of_a_cache_that_are_out_of_range_are_clamped_and_reported():
             values = values.dequantize() if isinstance(values, tb.MxTensor) else values
             assert bool(values[1].any()) == (size > 0)
             cache.status.zero_()
+
+
+def test_a_feature_loader_whose_consumer_changes_streams():
+    """The last batch is read on a busy stream; what the first stream allocates meanwhile does not touch its indices."""
+    n, dim = 4096, 32
+    loader = tb.CudaFeatureLoader(n, 1, dim, n // 2, format="mxfp8", shuffle=True, dtype=torch.float32, return_indices=True)
+    x = torch.randn(n, 1, dim, device="cuda")
+    loader.write(np.arange(n), x)
+    want = loader.cache.read(None, torch.float32)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    batches = iter(loader)
+    next(batches)
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        batch, index = next(batches)
+    at = index.cpu()
+    del index
+    assert next(batches, None) is None                    # the epoch's order is free now
+    del batches
+    filler = [torch.full((n,), -1, dtype=torch.int64, device="cuda") for _ in range(4)]
+    torch.cuda.synchronize()
+    assert torch.equal(batch, want[at.cuda()]) and loader.device_status() == 0 and len(filler) == 4
 
 
 # ---- scales on the device that change --------------------------------------------------------------------------

@@ -10,7 +10,7 @@ from __future__ import annotations
 import numpy as np
 
 from . import ops
-from .mx import MxCache, _dtype_id
+from .mx import MxCache, _dtype_id, _raw_stream
 
 __all__ = ["CudaFeatureLoader"]
 
@@ -113,11 +113,14 @@ class CudaFeatureLoader:
     def __iter__(self):
         torch = self._torch
         order = torch.from_numpy(self.epoch_order()).to(self._device)
+        made_on = _raw_stream(self._device.index)
         start = self._resume_batches
         self._resume_batches = 0
         self._batches_served = start
         for b in range(start, len(self)):
             index = order[b * self.batch_size:(b + 1) * self.batch_size]
+            if _raw_stream(self._device.index) != made_on:  # the consumer changed streams: the order outlives its reads there too
+                order.record_stream(torch.cuda.current_stream(self._device))
             batch = self.cache.read_mx(index) if self.output == "mx" else self.cache.read(index, self.dtype)
             items = list(batch) if isinstance(batch, tuple) else [batch]
             if self._labels is not None:
