@@ -424,7 +424,8 @@ TLB_API int tlb_mx_read_codes(const tlb_mx_cache* cache, const int64_t* index, i
                               uint8_t* scales, int32_t* lengths_out, void* stream);
 
 /* out (a.rows, b.rows) packed = values(a) * values(b)^T, sums in fp32, rounded once.  a and b have the
- * same format and cols.  workspace: tlb_mx_matmul_workspace bytes (0: NULL will do), 256-byte aligned,
+ * same format and cols.  The sums are those of the codes and block scales; the product of the two tensor scales
+ * (which multiplies them) must be a normal fp32 number.  workspace: tlb_mx_matmul_workspace bytes (0: NULL will do), 256-byte aligned,
  * used by this call alone until its work has ended. */
 TLB_API int64_t tlb_mx_matmul_workspace(const tlb_mx_rows* a, const tlb_mx_rows* b, int32_t out_dtype);
 TLB_API int tlb_mx_matmul(const tlb_mx_rows* a, const tlb_mx_rows* b, void* out, int32_t out_dtype, void* workspace,

@@ -237,3 +237,18 @@ def test_fill_refuses_loaders_that_leave_samples_out(monkeypatch):
                    [batch, batch]):
         assert loader.fill(images, lambda x: x) == 8
     assert len(written) == 6
+
+
+@pytest.mark.parametrize("a,b", [(1e30, 1e30), (1e-30, 1e-30), (2.0 ** -100, 2.0 ** -27), (2.0 ** 127, 2.0)])
+def test_tensor_scales_whose_product_leaves_the_range_are_refused(a, b):
+    """They would turn sums of zero into NaN, or everything into zero."""
+    from turboloader_b200 import _capi
+
+    lib = _capi.load()
+    rows = [_capi.MxRows(0x1000, 0x2000, 8, 64, 0, s, None) for s in (a, b)]
+    ready = (0x9000, 1 << 20, None)
+    assert lib.tlb_mx_matmul(*rows, 0x8000, 0, *ready) == 1 and b"scales" in lib.tlb_last_error()
+    assert lib.tlb_mx_linear(rows[0], 0x5000, 0, 64, rows[1], 0x6000, 0, 64, 0x8000, 0, *ready) == 1
+    assert lib.tlb_mx_matmul_workspace(*rows, 0) == -1
+    rows[1].scale = 1.0
+    assert lib.tlb_mx_matmul_workspace(*rows, 0) > 0

@@ -100,6 +100,7 @@ int check_product(const tlb_mx_rows* a, const tlb_mx_rows* b, int out_dtype) {
     if (int rc = check_rows(b, "b")) return rc;
     if (a->format != b->format) return fail(TLB_ERR_INVALID_ARG, "a and b must have the same format");
     if (a->cols != b->cols) return fail(TLB_ERR_INVALID_ARG, "a has %d columns, b has %d", a->cols, b->cols);
+    if (!std::isnormal(a->scale * b->scale)) return fail(TLB_ERR_INVALID_ARG, "the product of the tensor scales, %g and %g, leaves fp32's range", a->scale, b->scale);
     if (b->rows > TLB_MX_MAX_COLS) return fail(TLB_ERR_TOO_LARGE, "b: %lld rows exceed %d", static_cast<long long>(b->rows), TLB_MX_MAX_COLS);
     return check_dtype(out_dtype, "out");
 }
