@@ -438,7 +438,7 @@ TLB_API int tlb_mx_linear(const tlb_mx_rows* a, const void* x, int32_t x_dtype, 
                           int64_t workspace_bytes, void* stream);
 
 /* Products and gradients on the current device since the library was loaded whose kernels gave up a
- * bounded wait (seconds without progress) and left their result incomplete: 0 in a healthy process.
+ * bounded wait (seconds without progress): 0 in a healthy process.  What such a kernel has not summed is NaN.
  * Synchronises. */
 TLB_API int tlb_mx_incomplete(uint32_t* count);
 

@@ -73,6 +73,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
     __shared__ unsigned long long bars[2 * kMaxStages + 5];
     __shared__ unsigned tmem_base;
     __shared__ int gave_up;
+    __shared__ Pair pair;
     const unsigned smem = (smem_u32(raw) + 1023u) & ~1023u;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
     const unsigned rank = __shfl_sync(0xffffffffu, cluster_rank(), 0);
@@ -92,6 +93,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
         }
         mbar_init(drained, 1);
         gave_up = 0;
+        pair.gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         tma_prefetch_map(&gp.map_a);
         tma_prefetch_map(&gp.map_b);
@@ -104,11 +106,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
     tc_fence_after();
     const unsigned tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
     volatile int* stop = &gave_up;
+    const unsigned copied = b_boxes * kBoxB + gp.rows_a * (gp.transpose ? 256u : 128u);  // bytes of a stage, of each CTA
     wait_for_previous();
 
     if (warp == 0) {
         const bool issue = elect_one();
-        const unsigned full_at = at_leader(full), bytes = stage_bytes - kStageA + gp.rows_a * (gp.transpose ? 256u : 128u);
+        const unsigned full_at = at_leader(full);
         Ring r;
         unsigned started = 0;
         bool ok = true;
@@ -121,7 +124,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
                 if (!ok) break;
                 if (issue) {
                     const unsigned a = smem + r.s * stage_bytes, b = a + kStageA, bar = full_at + 8 * r.s;
-                    if (rank == 0) mbar_arrive_tx(full + 8 * r.s, 2 * bytes);
+                    if (rank == 0) mbar_arrive_tx(full + 8 * r.s, 2 * copied);
                     if (gp.transpose) {  // terms are stacked along g's rows, which the sum runs over
                         const int row = term * static_cast<int>(gp.sum) + at * kDepth;
                         tma_load_2d(a, &gp.map_a, m0, row, bar);
@@ -137,13 +140,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
                 if (++at == gp.term_stages) at = 0, ++term;
             }
         }
-        if (*stop && rank == 0) {  // every copy that was started lands before the pair ends
-            int none = 0;
-            for (unsigned j = 0; j < ring && j < started; ++j) {
-                r.back(ring);
-                mbar_wait(full + 8 * r.s, r.parity, &none);
-            }
-        }
+        if (issue) store_at(at_leader(smem_u32(&pair.started[rank][0])), started);
     } else if (warp == 1 && rank == 0) {
         const bool issue = elect_one();
         // bits 4-5 fp32 sums, 7-9 / 10-12 bf16, 15 / 16 A / B with the sum across rows, 17-22 N / 8, 24-28 M / 16
@@ -179,12 +176,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
                 }
             }
         }
-        if (*stop) {  // the instructions issued so far are done before TMEM is freed
-            int none = 0;
-            if (issue) tc_commit(drained);
-            __syncwarp();
-            mbar_wait(drained, 0, &none);
-        }
     } else if (warp >= 4) {
         const int quarter = warp % 4, half = (warp - 4) / 4;
         const unsigned staging = smem + kRing + (warp - 4) * kStaging;
@@ -193,13 +184,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
         const unsigned long long policy = store_policy(false);
         unsigned count = 0;
         const unsigned lanes = tmem + (static_cast<unsigned>(quarter * 32) << 16);
-        bool ok = true;
-        for (int it = first_item; ok && it < items; it += step) {
-            const Item item(gp, it);
+        const auto place = [&](const Item& item) {
             const long long in_part = static_cast<long long>(2 * item.m + rank) * kTileM + quarter * 32;
             const int n0 = item.n * gp.tile_n;
-            const TileOut<T> to{&gp.map_out, static_cast<T*>(gp.out), gp.pitch, item.split * (static_cast<long long>(gp.m_tiles) * 2 * kTileM) + in_part,
-                                gp.splits > 1 ? 32 : static_cast<int>(min(32ll, gp.rows - in_part)), n0, min(gp.tile_n, gp.cols - n0), gp.vec_ok, policy};
+            return TileOut<T>{&gp.map_out, static_cast<T*>(gp.out), gp.pitch, item.split * (static_cast<long long>(gp.m_tiles) * 2 * kTileM) + in_part,
+                              gp.splits > 1 ? 32 : static_cast<int>(min(32ll, gp.rows - in_part)), n0, min(gp.tile_n, gp.cols - n0), gp.vec_ok, policy};
+        };
+        bool ok = true;
+        int it = first_item;
+        for (; it < items; it += step) {
+            const Item item(gp, it);
             TileSum<T> sum;
             for (int from = item.first; from < item.last; from += gp.hold, ++count) {
                 const unsigned buf = count & 1;
@@ -209,14 +203,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grad_ke
                 sum.add(lanes + buf * 256, gp.tile_n, half, lane, acc_empty_at + 8 * buf);
             }
             if (!ok) break;
-            sum.write(to, gp.tile_n, half, lane, staging, alpha);
+            sum.write(place(item), gp.tile_n, half, lane, staging, alpha);
         }
+        for (; it < items; it += step) write_nan(place(Item(gp, it)), half);  // given up
         if (lane == 0) tma_store_wait_read();
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    cluster_sync();  // neither CTA's memory or barriers are used by the other any more
+    if (threadIdx.x == 0 && gave_up)
+        for (unsigned r = 0; r < 2; ++r) store_at(at_rank(smem_u32(&pair.gave_up), r), 1u);
+    __syncwarp();
+    cluster_sync();  // neither CTA's memory or barriers are used by the other any more, unless one gave up:
+    if (pair.gave_up) {
+        if (rank == 0 && warp == 0) wait_for_copies(full, ring, pair.started[0][0], pair.started[1][0], copied);
+        if (rank == 0 && warp == 1) {  // the instructions issued so far are done before TMEM is freed
+            int none = 0;
+            if (elect_one()) tc_commit(drained);
+            mbar_wait(drained, 0, &none);
+        }
+        __syncwarp();
+        cluster_sync();
+    }
     tc_fence_after();
     if (warp == 1) tmem_free(tmem, kTmemColumns);
     if (threadIdx.x == 0 && gave_up) atomicAdd(&g_gave_up, 1u);

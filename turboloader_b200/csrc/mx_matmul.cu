@@ -156,6 +156,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
     __shared__ unsigned long long bars[2 * kStagesB + 4 + 2 * kSlots + 1];
     __shared__ unsigned tmem_base;
     __shared__ int gave_up;
+    __shared__ Pair pair;
     const unsigned smem = (smem_u32(raw) + 1023u) & ~1023u;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
     const unsigned rank = __shfl_sync(0xffffffffu, cluster_rank(), 0);
@@ -184,6 +185,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
         }
         mbar_init(drained, 1);
         gave_up = 0;
+        pair.gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         tma_prefetch_map(&tp.map_a);
         tma_prefetch_map(&tp.map_b);
@@ -198,6 +200,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
     tc_fence_after();
     const unsigned tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
     volatile int* stop = &gave_up;
+    const unsigned a_bytes = tp.rows_a * 128 + kWords<FMT> * 512;  // of a stage's A, and of what comes through the ring
+    const unsigned ring_bytes = tile_n / 2 * 128 + kWords<FMT> * tp.groups_n * 512 + (tp.resident ? 0u : a_bytes);
     wait_for_previous();
 
     // Warps 0 and 1 walk their loops whole, so that addresses and descriptors are uniform; one lane issues.  (With a
@@ -206,8 +210,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
     if (warp == 0) {
         const bool issue = elect_one();
         Ring r;
-        unsigned rows = 0, started = 0;
-        const unsigned b_bytes = tile_n / 2 * 128 + kWords<FMT> * tp.groups_n * 512, a_bytes = tp.rows_a * 128 + kWords<FMT> * 512;
+        unsigned rows = 0, started = 0, started_a = 0;
         const unsigned full_at = at_leader(full), a_full_at = at_leader(a_full);
         int last_m = -1;
         bool ok = true;
@@ -232,12 +235,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
                         tma_load_2d(a + kCodesA, &tp.map_sa, 0, sa_row, bar);
                     }
                     __syncwarp();
+                    ++started_a;
                 }
                 ok = mbar_wait(empty + 8 * r.s, r.parity ^ 1, stop);
                 if (!ok) break;
                 if (issue) {
                     const unsigned b = b_base + r.s * b_step, bar = full_at + 8 * r.s;
-                    if (rank == 0) mbar_arrive_tx(full + 8 * r.s, 2 * (b_bytes + (tp.resident ? 0u : a_bytes)));
+                    if (rank == 0) mbar_arrive_tx(full + 8 * r.s, 2 * ring_bytes);
                     tma_load_2d(b, &tp.map_b, kt * 128, n * tile_n + static_cast<int>(rank) * (tile_n / 2), bar);
                     tma_load_2d(b + kCodesB, &tp.map_sb, 0, (n * tp.k_stages + kt) * kWords<FMT> * tp.groups_n, bar);
                     if (!tp.resident) {
@@ -251,13 +255,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
                 ++started;
             }
         }
-        if (*stop && rank == 0) {  // every copy that was started lands before the pair ends
-            int none = 0;
-            for (unsigned j = 0; j < ring && j < started; ++j) {
-                r.back(ring);
-                mbar_wait(full + 8 * r.s, r.parity, &none);
-            }
-            for (int kt = 0; rows && kt < tp.k_stages; ++kt) mbar_wait(a_full + 8 * kt, (rows - 1) & 1, &none);
+        if (issue) {
+            store_at(at_leader(smem_u32(&pair.started[rank][0])), started);
+            store_at(at_leader(smem_u32(&pair.started[rank][1])), started_a);
         }
     } else if (warp == 1 && rank == 0) {
         const bool issue = elect_one();
@@ -315,12 +315,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
                 }
             }
         }
-        if (*stop) {  // the instructions issued so far are done before TMEM is freed
-            int none = 0;
-            if (issue) tc_commit(drained);
-            __syncwarp();
-            mbar_wait(drained, 0, &none);
-        }
     } else if (warp >= 4) {
         const int quarter = warp % 4, half = (warp - 4) / 4;
         const unsigned staging = smem + kRing + (warp - 4) * kStaging;
@@ -330,14 +324,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
         const unsigned long long policy = store_policy(tp.passing);
         unsigned count = 0;
         const unsigned lanes = tmem + (static_cast<unsigned>(quarter * 32) << 16);
-        bool ok = true;
-        for (Walk w(tp); ok && w.tile < w.end; w.tile += w.step) {
+        const auto place = [&](const Walk& w) {
             int m, n;
             w.place(tp, m, n);
             const long long m0 = static_cast<long long>(2 * m + rank) * kTileM + quarter * 32;
             const int n0 = n * tile_n;
-            const TileOut<T> to{&tp.map_out, static_cast<T*>(p.out), n_all, m0, static_cast<int>(min(32ll, p.a.rows - m0)), n0, min(tile_n, n_all - n0),
-                                tp.vec_ok, policy};
+            return TileOut<T>{&tp.map_out, static_cast<T*>(p.out), n_all, m0, static_cast<int>(min(32ll, p.a.rows - m0)), n0, min(tile_n, n_all - n0),
+                              tp.vec_ok, policy};
+        };
+        bool ok = true;
+        Walk w(tp);
+        for (; w.tile < w.end; w.tile += w.step) {
+            const TileOut<T> to = place(w);
             if constexpr (LONG) {
                 TileSum<T> sum;
                 for (int from = 0; from < tp.k_stages; from += hold, ++count) {
@@ -347,7 +345,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
                     tc_fence_after();
                     sum.add(lanes + buf * kMaxTileN, tile_n, half, lane, acc_empty_at + 8 * buf);
                 }
-                if (ok) sum.write(to, tile_n, half, lane, staging, alpha);
+                if (!ok) break;
+                sum.write(to, tile_n, half, lane, staging, alpha);
             } else {
                 const unsigned buf = count & 1;
                 ok = mbar_wait(acc_full + 8 * buf, (count >> 1) & 1, stop);
@@ -357,12 +356,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
                 ++count;
             }
         }
+        for (; w.tile < w.end; w.tile += w.step) write_nan(place(w), half);  // given up
         if (lane == 0) tma_store_wait_read();
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    cluster_sync();  // neither CTA's memory or barriers are used by the other any more
+    if (threadIdx.x == 0 && gave_up)
+        for (unsigned r = 0; r < 2; ++r) store_at(at_rank(smem_u32(&pair.gave_up), r), 1u);
+    __syncwarp();
+    cluster_sync();  // neither CTA's memory or barriers are used by the other any more, unless one gave up:
+    if (pair.gave_up) {
+        if (rank == 0 && warp == 0) {
+            wait_for_copies(full, ring, pair.started[0][0], pair.started[1][0], ring_bytes);
+            if (tp.resident) wait_for_copies(a_full, tp.k_stages, pair.started[0][1], pair.started[1][1], a_bytes);
+        }
+        if (rank == 0 && warp == 1) {  // the instructions issued so far are done before TMEM is freed
+            int none = 0;
+            if (elect_one()) tc_commit(drained);
+            mbar_wait(drained, 0, &none);
+        }
+        __syncwarp();
+        cluster_sync();
+    }
     tc_fence_after();
     if (warp == 1) tmem_free(tmem, kTmemColumns);
     if (threadIdx.x == 0 && gave_up) atomicAdd(&g_gave_up, 1u);

@@ -12,10 +12,6 @@ struct Ring {
     __device__ void next(unsigned stages) {
         if (++s == stages) s = 0, parity ^= 1u;
     }
-    __device__ void back(unsigned stages) {
-        if (s == 0) s = stages, parity ^= 1u;
-        --s;
-    }
 };
 
 constexpr int kStaging = 32 * 128;  // an epilogue warp's 32 rows of 128 bytes
@@ -87,6 +83,22 @@ __device__ __forceinline__ void write_chunk(const TileOut<T>& to, const float* v
                 }
             }
     }
+}
+
+// NaN instead of a warp's part of a tile whose sums were given up: rows x width values, every second chunk of 128 bytes of
+// a row from this one on.  (A call, so that it takes no registers from the epilogue.)
+template <typename T>
+__device__ __noinline__ void fill_nan(T* out, long long pitch, int rows, int width) {
+    constexpr int chunk = 128 / sizeof(T);
+    const int lane = threadIdx.x % 32;
+    for (int r = 0; r < rows; ++r)
+        for (int c0 = 0; c0 < width; c0 += 2 * chunk)
+            for (int c = c0 + lane; c < min(c0 + chunk, width); c += 32) out[r * pitch + c] = from_float<T>(__uint_as_float(0x7fffffffu));
+}
+template <typename T>
+__device__ __forceinline__ void write_nan(const TileOut<T>& to, int half) {
+    constexpr int chunk = 128 / sizeof(T);
+    fill_nan(to.out + to.m0 * to.pitch + to.n0 + half * chunk, to.pitch, to.rows, to.width - half * chunk);
 }
 
 // The tensor cores cut where they add to an accumulator, by up to 2^-23 of the partial sum for each instruction and always

@@ -19,11 +19,12 @@ __device__ __forceinline__ bool elect_one() {  // one lane of a converged warp
 __device__ __forceinline__ void mbar_init(unsigned bar, unsigned count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
-__device__ __forceinline__ void mbar_arrive(unsigned bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
 __device__ __forceinline__ void mbar_arrive_tx(unsigned bar, unsigned bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// Counts bytes as landed that no copy will bring.
+__device__ __forceinline__ void mbar_complete_tx(unsigned bar, unsigned bytes) {
+    asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ bool mbar_try(unsigned bar, unsigned parity) {
     unsigned done;
@@ -37,20 +38,18 @@ __device__ __forceinline__ unsigned long long now_ns() {
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
     return t;
 }
-// Waits for a phase; false when the wait was given up, here or by another warp of the CTA.  A CTA that
-// gave up ends in order: every role leaves its loop, copies in flight are waited for, TMEM is freed.
+// Waits for a phase, a whole warp together; false (in all lanes) when the wait was given up, here or by another warp of
+// the CTA.  A CTA that gave up ends in order: every role leaves its loop, what it has not summed is written as NaN,
+// copies in flight are waited for (Pair), TMEM is freed.
 __device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity, volatile int* gave_up) {
-    if (mbar_try(bar, parity)) return true;
+    if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
     const unsigned long long began = now_ns();
     for (;;) {
 #pragma unroll 1
         for (int i = 0; i < 64; ++i)
-            if (mbar_try(bar, parity)) return true;
-        if (*gave_up) return false;
-        if (now_ns() - began > kGiveUpNs) {
-            *gave_up = 1;
-            return false;
-        }
+            if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
+        if (now_ns() - began > kGiveUpNs) *gave_up = 1;
+        if (__any_sync(0xffffffffu, *gave_up)) return false;
     }
 }
 
@@ -61,16 +60,41 @@ __device__ __forceinline__ unsigned cluster_rank() {
     asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
     return r;
 }
-__device__ __forceinline__ unsigned at_leader(unsigned addr) {
+__device__ __forceinline__ unsigned at_rank(unsigned addr, unsigned rank) {
     unsigned a;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(addr));
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
     return a;
+}
+__device__ __forceinline__ unsigned at_leader(unsigned addr) { return at_rank(addr, 0); }
+__device__ __forceinline__ void store_at(unsigned cluster_addr, unsigned v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
 }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void mbar_arrive_at(unsigned cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// What the CTAs of a pair tell each other for their end, in the shared memory of both (the counts in the leader's).
+struct Pair {
+    unsigned gave_up;         // one of them did
+    unsigned started[2][2];   // copies that each rank started: into the ring, and of A into its slots
+};
+// Waits for the copies that either rank of the pair started and that nothing has waited for: the last ones round a
+// ring of barriers that count a share of each rank.  A copy that one rank started and the other did not is made whole:
+// the leader's arrival, or the missing share.  A warp of the leader, after the pair has met.
+__device__ __forceinline__ void wait_for_copies(unsigned bars, unsigned ring, unsigned mine, unsigned other, unsigned share) {
+    int none = 0;
+    const bool one = elect_one();
+    const unsigned most = mine > other ? mine : other;
+    for (unsigned j = most > ring ? most - ring : 0; j < most; ++j) {
+        const unsigned bar = bars + 8 * (j % ring);
+        if (one && j >= mine) mbar_arrive_tx(bar, share);
+        else if (one && j >= other) mbar_complete_tx(bar, share);
+        __syncwarp();
+        mbar_wait(bar, (j / ring) & 1, &none);
+    }
 }
 // A box of a 2-D map into this CTA's shared memory, counted on a barrier of this CTA or of the leader.
 __device__ __forceinline__ void tma_load_2d(unsigned dst, const CUtensorMap* map, int x, int y, unsigned bar) {

@@ -301,8 +301,8 @@ def mx_matmul(a, b, dtype=torch.bfloat16, *, out=None, stream=None):
 
 
 def mx_incomplete() -> int:
-    """Products and gradients on the current device whose kernels gave up a bounded wait and left their result
-    incomplete, since the library was loaded (synchronises): 0 in a healthy process."""
+    """Products and gradients on the current device whose kernels gave up a bounded wait and left NaN where they had not
+    summed, since the library was loaded (synchronises): 0 in a healthy process."""
     count = C.c_uint32(0)
     _capi.check(_capi.load().tlb_mx_incomplete(C.byref(count)))
     return int(count.value)
