@@ -26,6 +26,12 @@ class _Library:
     def tlb_mx_read_codes(self, *a):
         return 0
 
+    def tlb_mx_read(self, *a):
+        return 0
+
+    def tlb_mx_matmul(self, *a):
+        return 0
+
     def tlb_mx_linear(self, *a):
         return 0
 
@@ -200,6 +206,38 @@ def test_only_rows_that_the_gradients_read_are_saved(library, x_held, w_held, x_
         mx.mx_linear(operand(2, x_held, x_grad), operand(3, w_held, w_grad), "nvfp4")
     size = {2: 1024 + 256, 3: 1536 + 256} if not (x_held or w_held) else {2: 2 * 576, 3: 3 * 576}  # parts of a buffer start at multiples of 256
     assert sum(saved) == (size[2] if w_grad else 0) + (size[3] if x_grad else 0)
+
+
+def _rows(*lead, cols=64):
+    return mx.MxTensor(torch.zeros(*lead, 64, dtype=torch.uint8), torch.zeros(*lead, 8, dtype=torch.uint8), (*lead, cols), "nvfp4")
+
+
+@pytest.mark.parametrize("call", [lambda out: mx.mx_dequantize(_rows(4), out=out), lambda out: mx.mx_matmul(_rows(4), _rows(64), torch.float32, out=out),
+                                  lambda out: mx.MxCache(_rows(4, 1).codes, _rows(4, 1).scales, 64, "nvfp4").read(None, torch.float32, out=out.view(4, 1, 64))])
+def test_writes_into_a_tensor_that_a_graph_saved_are_seen(library, call):
+    out = torch.zeros(4, 64)
+    w = torch.ones(64, requires_grad=True)
+    call(out)
+    (out * w).sum().backward()
+    y = (out * w).sum()
+    call(out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    out.requires_grad_(True)
+    with pytest.raises(ValueError, match="gradients"):
+        call(out)
+    with torch.no_grad():
+        call(out)
+
+
+def test_a_cache_written_before_the_gradients_of_its_rows_is_seen(library):
+    codes, scales = torch.zeros(4, 1, 64, dtype=torch.uint8), torch.zeros(4, 1, 8, dtype=torch.uint8)
+    cache = mx.MxCache(codes, scales, 64, "nvfp4")
+    w = torch.randn(5, 64, requires_grad=True)
+    y = mx.mx_linear(mx.MxTensor(codes, scales, (4, 1, 64), "nvfp4"), w, "nvfp4")
+    cache.write(torch.arange(2), torch.zeros(2, 1, 64))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
 
 
 # ---- the loader --------------------------------------------------------------------------------------------------

@@ -251,6 +251,9 @@ def _out(out, shape, dtype, device):
         raise ValueError(f"out must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}")
     if out.data_ptr() % 16:
         raise ValueError("out must be 16-byte aligned")
+    if out.requires_grad and torch.is_grad_enabled():
+        raise ValueError("out must not require gradients")
+    torch.autograd.graph.increment_version(out)  # torch does not see the kernel's writes; a graph that saved it has to
     return out
 
 
@@ -544,6 +547,7 @@ class MxCache:
                 return self.write(index, x, lengths=lengths)
         # The claims of a long write are this call's own: writes on several streams share nothing but the rows.
         owner = torch.full((max(self.slots, 1),), -1, dtype=torch.int32, device=device) if n > _capi.MX_SCAN_SAMPLES else None
+        torch.autograd.graph.increment_version([self.codes, self.scales] if self.lengths is None else [self.codes, self.scales, self.lengths])
         _capi.check(_capi.load().tlb_mx_write(self._struct(owner), index.data_ptr(), n, x.data_ptr(), dt, x.stride(1), x.stride(0),
                                               None if lengths is None else lengths.data_ptr(), _raw_stream(device.index)))
 
