@@ -15,7 +15,7 @@
 namespace tlb {
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kThreads = 128, kRows = 2;  // rows of the matrix a warp takes
 
 __device__ __forceinline__ void e2m1_pairs(unsigned codes, __half2 v[4]) {
     unsigned h[4];
@@ -42,28 +42,28 @@ __device__ __forceinline__ float add_scaled(float sum, float a, float b, float a
     return __fmaf_rn(__fmul_rn(sum, fminf(a, b)), larger, acc);
 }
 
-template <typename T, int FMT, int ROWS, int FEW>
+template <typename T, int FMT, int FEW>
 __global__ void __launch_bounds__(kThreads) few_kernel(MxProduct p) {
     const int lane = threadIdx.x % 32;
     const int n_all = static_cast<int>(p.b.rows), few = static_cast<int>(p.a.rows);
-    const int n0 = (blockIdx.x * (kThreads / 32) + threadIdx.x / 32) * ROWS;
+    const int n0 = (blockIdx.x * (kThreads / 32) + threadIdx.x / 32) * kRows;
     if (n0 >= n_all) return;
     const int code_pitch = mx_code_pitch(FMT, p.a.cols), scale_pitch = mx_scale_pitch(FMT, p.a.cols);
-    const unsigned char *codes[ROWS], *scales[ROWS];
+    const unsigned char *codes[kRows], *scales[kRows];
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) {  // a row behind the last is read again in its place, and not written
+    for (int r = 0; r < kRows; ++r) {  // a row behind the last is read again in its place, and not written
         const long long row = min(n0 + r, n_all - 1);
         codes[r] = p.b.codes + row * code_pitch;
         scales[r] = p.b.scales + row * scale_pitch;
     }
-    float acc[ROWS][FEW] = {};
+    float acc[kRows][FEW] = {};
     const int pieces = code_pitch / 16;
 #pragma unroll 4
     for (int piece = lane; piece < pieces; piece += 32) {
-        uint4 w[ROWS];
-        unsigned ws[ROWS];
+        uint4 w[kRows];
+        unsigned ws[kRows];
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) {
+        for (int r = 0; r < kRows; ++r) {
             w[r] = __ldg(reinterpret_cast<const uint4*>(codes[r]) + piece);
             ws[r] = scale_bits<FMT>(scales[r], piece);
         }
@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(kThreads) few_kernel(MxProduct p) {
                 for (int i = 0; i < 4; ++i) e4m3_values(xw[i], xv + 4 * i);
                 const float s = e8m0_value(xs);
 #pragma unroll
-                for (int r = 0; r < ROWS; ++r) {
+                for (int r = 0; r < kRows; ++r) {
                     const unsigned ww[4] = {w[r].x, w[r].y, w[r].z, w[r].w};
                     float sum = 0.0f;
 #pragma unroll
@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kThreads) few_kernel(MxProduct p) {
                 for (int i = 0; i < 4; ++i) e2m1_pairs(xw[i], xv + 4 * i);
                 const float s0 = FMT == kNvfp4 ? e4m3_value(xs & 0xffu) : e8m0_value(xs), s1 = FMT == kNvfp4 ? e4m3_value(xs >> 8) : s0;
 #pragma unroll
-                for (int r = 0; r < ROWS; ++r) {
+                for (int r = 0; r < kRows; ++r) {
                     const unsigned ww[4] = {w[r].x, w[r].y, w[r].z, w[r].w};
                     float part[2];
 #pragma unroll
@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kThreads) few_kernel(MxProduct p) {
     }
     const float alpha = __fmul_rn(mx_tensor_scale(p.a), mx_tensor_scale(p.b));
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r)
+    for (int r = 0; r < kRows; ++r)
 #pragma unroll
         for (int m = 0; m < FEW; ++m) {
             if (m >= few) break;
@@ -138,10 +138,11 @@ __global__ void __launch_bounds__(kThreads) few_kernel(MxProduct p) {
 template <typename T, int FMT>
 void launch(const MxProduct& p, cudaStream_t st) {
     const int n = static_cast<int>(p.b.rows);
-    auto grid = [&](int rows) { return static_cast<unsigned>((n + rows * (kThreads / 32) - 1) / (rows * (kThreads / 32))); };
-    if (p.a.rows == 1) few_kernel<T, FMT, 2, 1><<<grid(2), kThreads, 0, st>>>(p);
-    else if (p.a.rows == 2) few_kernel<T, FMT, 2, 2><<<grid(2), kThreads, 0, st>>>(p);
-    else few_kernel<T, FMT, 2, 4><<<grid(2), kThreads, 0, st>>>(p);
+    constexpr int cta_rows = kRows * (kThreads / 32);
+    const unsigned grid = static_cast<unsigned>((n + cta_rows - 1) / cta_rows);
+    if (p.a.rows == 1) few_kernel<T, FMT, 1><<<grid, kThreads, 0, st>>>(p);
+    else if (p.a.rows == 2) few_kernel<T, FMT, 2><<<grid, kThreads, 0, st>>>(p);
+    else few_kernel<T, FMT, 4><<<grid, kThreads, 0, st>>>(p);
 }
 
 template <typename T>
