@@ -391,7 +391,7 @@ TLB_API int64_t tlb_mx_scale_pitch(int32_t format, int32_t cols);  /* bytes, or 
 
 /* x (rows, cols) of x_dtype, x_pitch elements between rows -> q.  All entry points of this section
  * enqueue on `stream`, on the current device, allocate nothing, do not synchronise and may be captured
- * into a CUDA graph. */
+ * into a CUDA graph.  What they read and write packed (out, g, grad_a, grad_b, codes) starts on a 16-byte boundary. */
 TLB_API int tlb_mx_quantize(const tlb_mx_rows* q, const void* x, int32_t x_dtype, int64_t x_pitch, void* stream);
 
 /* A cache: rows.rows = slots * tokens.  One sample fills one slot. */
