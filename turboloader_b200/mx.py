@@ -229,7 +229,8 @@ def mx_quantize(x, format="nvfp4", *, scale=1.0, stream=None):
     """``x`` (..., cols), float32, bfloat16 or float16, as an ``MxTensor``.  The values of a row must be
     contiguous and the rows equally spaced (a slice of a wider matrix will do).  ``scale``: the tensor scale
     that values are divided by first, a float or one float32 value on the device (copied: the result keeps the
-    value of this call); a power of two loses nothing.  For ``nvfp4``, ``max|x| / 2688`` rounded up to a power of two uses the range of its scales."""
+    value of this call); a power of two loses nothing.  For ``nvfp4``, ``max|x| / 2688`` rounded up to a power of
+    two uses the range of its scales."""
     fmt = _format_id(format)
     rows, _, pitch = _as_rows(x, "x")
     dt = _dtype_id(x.dtype, "x")
