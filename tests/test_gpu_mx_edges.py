@@ -104,6 +104,8 @@ def test_a_first_long_write_that_is_captured():
         got = cache.read(None, torch.float32).view(slots, cols)
         assert torch.equal(got[:3], want[:3]) and torch.equal(got[3], want[599]) and torch.equal(got[4:599], want[4:599])
         assert not got[599:].any()
+        cache.write(index, x.flip(1) * 3)               # one that is not captured, between replays
+        assert torch.equal(cache.read(index[:3], torch.float32).view(3, cols), tb.mx_quantize(x[:3].view(3, cols) * 3).dequantize())
 
 
 def test_lengths_of_a_cache_that_are_out_of_range_are_clamped_and_reported():

@@ -113,23 +113,35 @@ def test_gradients_of_any_leading_dimensions_and_of_no_rows(library, lead, n):
     assert gx.shape == x.shape and gw.shape == w.shape
 
 
-def test_the_claims_of_a_write_are_its_own(library):
-    """No write sees words that another one, on another stream, may be claiming or has yet to fill."""
+def test_the_claims_of_a_write_belong_to_its_stream(library, monkeypatch):
+    """No write sees words that one on another stream may be claiming or has yet to fill, and a captured one fills its own."""
     cache = mx.MxCache(torch.zeros(700, 1, 64, dtype=torch.uint8), torch.zeros(700, 1, 8, dtype=torch.uint8), 40, "nvfp4")
-    seen = []
+    stream, capturing, seen = [0], [False], []
+    monkeypatch.setattr(mx, "_raw_stream", lambda index: stream[0])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+
+    def write(n, on, captured=False):
+        stream[0], capturing[0] = on, captured
+        cache.write(torch.arange(n), torch.zeros(n, 1, 40))
+        return seen[-1]
 
     def on_write(c):
-        words = (C.c_int32 * 700).from_address(c.owner)
-        seen.append(list(words))
-        words[:] = [5] * 700
+        words = (C.c_int32 * 700).from_address(c.owner) if c.owner else None
+        seen.append((c.owner, words and list(words)))
+        if words:
+            words[:] = [stream[0]] * 700
 
     library.on_write = on_write
-    for n in (257, 600):
-        cache.write(torch.arange(n), torch.zeros(n, 1, 40))
-    assert seen == [[-1] * 700] * 2
-    library.on_write = lambda c: seen.append(c.owner)
-    cache.write(torch.arange(256), torch.zeros(256, 1, 40))
-    assert seen[-1] is None
+    unused = [-1] * 700
+    assert write(256, 1) == (None, None)
+    at, words = write(257, 1)
+    assert words == unused
+    assert write(600, 2, captured=True)[1] == unused      # before the stream's first eager one
+    other, words = write(600, 2)
+    assert words == unused and other != at
+    assert write(300, 1) == (at, [1] * 700)               # the stream's own, in its order
+    captured, words = write(300, 1, captured=True)
+    assert words == unused and captured not in (at, other)
 
 
 def _value(address):

@@ -483,6 +483,7 @@ class MxCache:
 
     def __init__(self, codes, scales, cols, format, *, lengths=None, scale=1.0, status=None):
         self._fmt = _format_id(format)
+        self._owners = {}
         _cuda(codes, "codes")
         if codes.dim() != 3:
             raise ValueError("codes must be (slots, tokens, code pitch)")
@@ -546,11 +547,22 @@ class MxCache:
         if _away(device, stream):
             with _there(device, stream):
                 return self.write(index, x, lengths=lengths)
-        # The claims of a long write are this call's own: writes on several streams share nothing but the rows.
-        owner = torch.full((max(self.slots, 1),), -1, dtype=torch.int32, device=device) if n > _capi.MX_SCAN_SAMPLES else None
+        owner = self._claims() if n > _capi.MX_SCAN_SAMPLES else None
         torch.autograd.graph.increment_version([self.codes, self.scales] if self.lengths is None else [self.codes, self.scales, self.lengths])
         _capi.check(_capi.load().tlb_mx_write(self._struct(owner), index.data_ptr(), n, x.data_ptr(), dt, x.stride(1), x.stride(0),
                                               None if lengths is None else lengths.data_ptr(), _raw_stream(device.index)))
+
+    def _claims(self):
+        """The words that a long write decides with between samples naming the same slot, -1 each.  Every stream has its
+        own, so that writes on several streams share nothing but the rows; a captured write too, whose words are filled
+        when it is replayed."""
+        stream = _raw_stream(self.device.index)
+        owner = self._owners.get(stream)
+        if owner is None or torch.cuda.is_current_stream_capturing():
+            owner = torch.full((max(self.slots, 1),), -1, dtype=torch.int32, device=self.device)
+            if not torch.cuda.is_current_stream_capturing():
+                self._owners[stream] = owner
+        return owner
 
     def _picked(self, index):
         if index is None:
